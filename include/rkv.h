@@ -338,6 +338,35 @@ rkv_status rkv_prefill_q8(rkv_ctx *ctx, const rkv_kv_geometry *g, const void *pa
  * pointers in args are not read. */
 size_t rkv_prefill_workspace_bytes(const rkv_kv_geometry *g, const rkv_prefill_args *args);
 
+/* ---- 4-bit pages ------------------------------------------------------------
+ * The cache in 4 bits, half the bytes of Q8_0: 32 values of a row are E2M1
+ * codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign) times one power of two 2^e, 17
+ * bytes a block.  e is the smallest exponent with max|v| <= 7 * 2^e, kept
+ * within -24..15 for K and -22..7 for V; a code is v / 2^e rounded to nearest,
+ * ties to the even code, saturating at 6.  A block with a value that is not
+ * finite reads back as NaN.  Pages have the geometry, allocator, block tables
+ * and copy-on-write copies of the Q8_0 ones, with page_tokens 32, 64, 128 or
+ * 256 and rkv_mx4_page_bytes bytes; their layout is internal (rkv_append_rope
+ * writes and rkv_read_rows reads them).  No counterpart in the reference,
+ * whose flash decode reads Q8_0 only (har/shaders/flash_decode_q8.comp:1-25);
+ * har/crates/r4kv's own 4-bit format packs integer codes under an f16 scale. */
+size_t rkv_mx4_page_bytes(const rkv_kv_geometry *g);
+
+/* rkv_decode_q8 over 4-bit pages: the same arguments, workspace rules and
+ * faults, but args->append must be NULL (RKV_ERR_UNSUPPORTED; append with
+ * rkv_append_rope), and with partition_tokens 0 the device splits sequences
+ * longer than 512 tokens in whole multiples of 128 tokens.  A NaN block makes
+ * the rows that attend it NaN (a V block the dimensions it covers); rows that
+ * do not attend it are not touched by it. */
+rkv_status rkv_decode_mx4(rkv_ctx *ctx, const rkv_kv_geometry *g, const void *pages,
+                          const int32_t *block_tables, int32_t bt_stride,
+                          const int32_t *seq_lens, int32_t n_seqs,
+                          const rkv_decode_args *args, void *stream);
+/* Workspace bytes of rkv_decode_mx4: 0 where one partition covers every
+ * sequence (partition_tokens 0: up to a max_seq_len of 512); with
+ * partition_tokens 0 it does not fall as batch or max_seq_len grows. */
+size_t rkv_decode_mx4_workspace_bytes(const rkv_kv_geometry *g, const rkv_decode_args *args);
+
 /* Export seq's K or V cache in the reference contiguous layout
  * [kv_heads][len][head_dim/32*34] bytes (what flash_decode_reference reads,
  * attention.rs:144-147; row_to_words is a reinterpretation, :115-120). */

@@ -167,6 +167,10 @@ _SIGS = {
     "rkv_prefill_workspace_bytes": (C.c_size_t, [C.POINTER(Geometry), C.POINTER(PrefillArgs)]),
     "rkv_pool_prefill_workspace_bytes": (C.c_size_t, [P, C.POINTER(PrefillArgs)]),
     "rkv_decode_partition_tokens": (C.c_int32, [C.POINTER(Geometry), C.POINTER(DecodeArgs)]),
+    "rkv_mx4_page_bytes": (C.c_size_t, [C.POINTER(Geometry)]),
+    "rkv_decode_mx4": (C.c_int32, [P, C.POINTER(Geometry), P, P, C.c_int32, P, C.c_int32,
+                                   C.POINTER(DecodeArgs), P]),
+    "rkv_decode_mx4_workspace_bytes": (C.c_size_t, [C.POINTER(Geometry), C.POINTER(DecodeArgs)]),
     "rkv_decode_q8_partials": (C.c_int32, [P, C.POINTER(Geometry), P, P, C.c_int32, P,
                                            C.c_int32, C.POINTER(DecodeArgs), P, P, P]),
     "rkv_splitk_combine": (C.c_int32, [P, P, P, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
@@ -591,6 +595,22 @@ def decode_q8_noalloc(ctx: Ctx, g: Geometry, pages, block_tables, seq_lens, a: D
     check(lib().rkv_decode_q8_noalloc(ctx.h, C.byref(g), _ptr(pages), _ptr(block_tables),
                                       block_tables.shape[-1], _ptr(seq_lens), seq_lens.numel(),
                                       C.byref(a), _stream(stream)))
+
+
+def mx4_page_bytes(g: Geometry) -> int:
+    return lib().rkv_mx4_page_bytes(C.byref(g))
+
+
+def decode_mx4_workspace_bytes(g: Geometry, a: DecodeArgs) -> int:
+    return lib().rkv_decode_mx4_workspace_bytes(C.byref(g), C.byref(a))
+
+
+def decode_mx4(ctx: Ctx, g: Geometry, pages, block_tables, seq_lens, a: DecodeArgs,
+               stream=None) -> None:
+    """rkv_decode_q8 over 4-bit pages (a.append must be None)."""
+    check(lib().rkv_decode_mx4(ctx.h, C.byref(g), _ptr(pages), _ptr(block_tables),
+                               block_tables.shape[-1], _ptr(seq_lens), seq_lens.numel(),
+                               C.byref(a), _stream(stream)))
 
 
 def decode_q8_partials(ctx: Ctx, g: Geometry, pages, block_tables, seq_lens, a: DecodeArgs,

@@ -1849,10 +1849,10 @@ __device__ __forceinline__ int32_t wave_isum(int32_t v, int lane) {
 // sequence id and length), partition `part` of nb.  Every workgroup computes
 // the same length and the same order (entries in batch order, partitions in
 // token order), so workgroup x takes the x-th partition.  Returns false past
-// the last one.
+// the last one.  A partition spans at most 64 pages of page_tokens tokens.
 __device__ __forceinline__ bool locate(const DecodeLaunch &p, int lane, int32_t x, int32_t &pt,
                                        int32_t &b, int32_t &seq, int32_t &len, int32_t &part,
-                                       int32_t &nb) {
+                                       int32_t &nb, int32_t page_tokens) {
   constexpr int kCached = 4;  // entries < 256 stay in registers
   int32_t lc[kCached], sc[kCached];
 #pragma unroll
@@ -1898,7 +1898,7 @@ __device__ __forceinline__ bool locate(const DecodeLaunch &p, int lane, int32_t 
     // that span within the 64 page ids of a workgroup, else it rounds up to
     // 64 whole pages.  The rounding keeps the length monotone in k, so the
     // binary search below stays valid.
-    const int32_t PT = p.g.page_tokens;
+    const int32_t PT = page_tokens;
     auto len_of = [&](int32_t k) -> int32_t {
       const int32_t t = k * p.pt_unit;
       return (t % PT != 0 && t + PT - kTile > 64 * PT) ? 64 * PT : t;
@@ -1989,7 +1989,7 @@ __global__ __launch_bounds__(64 * NW, NW) void decode_kernel(DecodeLaunch p) {
   const Geo g = p.g;
 
   int32_t pt, b, seq, lenc, part, nb;
-  if (!locate(p, lane, (int32_t)blockIdx.x, pt, b, seq, lenc, part, nb)) return;
+  if (!locate(p, lane, (int32_t)blockIdx.x, pt, b, seq, lenc, part, nb, p.g.page_tokens)) return;
   // the combine finds entry b's partials through the header, written before
   // any check can end this workgroup
   if (p.ws_hdr != nullptr && kvh == 0 && threadIdx.x == 0) {

@@ -104,6 +104,16 @@ struct DecodeLaunch {
 // rows per kv head = q_len * q_heads / kv_heads must be <= 32
 hipError_t launch_decode(const DecodeLaunch &d, hipStream_t s);
 
+// The same over 4-bit pages (rkv_mx4.h), whose workgroups take a partition
+// with kMx4Waves waves, 32-token tiles in turn; part_tokens is a multiple of
+// 32, pt_unit one tile of every wave, and a partition may span any pages.
+// append, the per-entry partials layout and the LDS ring depth have no part in it.
+constexpr int kMx4Waves = 4;
+// Workgroups resident per CU: two waves a SIMD up to 16 rows per kv head (8
+// with an f32 query, which takes three times the registers), one above.
+constexpr int mx4_wgs_per_cu(int rows, bool q_bf16) { return rows > (q_bf16 ? 16 : 8) ? 1 : 2; }
+hipError_t launch_mx4_decode(const DecodeLaunch &d, hipStream_t s);
+
 // Chunked prefill attention: entry e holds rows[e] query rows of sequence
 // seq[e] at positions ctx[e] .. ctx[e]+rows[e]-1 (already appended), stored
 // at rows qoff[e].. of q/out ([rows][q_heads][head_dim]); row i attends

@@ -20,6 +20,7 @@
 #include "rkv_crc32c.h"
 #include "rkv_host.h"
 #include "rkv_launch.h"
+#include "rkv_mx4.h"
 
 using rkv::Geo;
 using rkv::host::fail;
@@ -74,6 +75,14 @@ rkv_status check_geometry(const rkv_kv_geometry *g, const char *op) {
     return fail(RKV_ERR_UNSUPPORTED, op, "page_tokens=%d (built: 16, 32, 64, 128, 256)",
                 g->page_tokens);
   if (g->num_pages < 1) return fail(RKV_ERR_INVALID_ARG, op, "num_pages=%d", g->num_pages);
+  return RKV_OK;
+}
+
+// 4-bit pages hold whole 32-token tiles.
+rkv_status check_mx4_geometry(const rkv_kv_geometry *g, const char *op) {
+  if (rkv_status s = check_geometry(g, op)) return s;
+  if (g->page_tokens < rkv::kMx4Tile)
+    return fail(RKV_ERR_UNSUPPORTED, op, "page_tokens=%d (built for 4-bit pages: 32, 64, 128, 256)", g->page_tokens);
   return RKV_OK;
 }
 
@@ -628,6 +637,36 @@ Plan plan_of(const rkv_kv_geometry *g, const rkv_decode_args *a, int32_t stages,
   return pl;
 }
 
+// The plan over 4-bit pages: partitions are whole rounds of a workgroup's
+// waves (one tile each) and may span any number of pages.  Up to kMx4Whole
+// rounds a sequence stays one partition, which its workgroup's waves share.
+constexpr int32_t kMx4Whole = 4;
+
+Plan mx4_plan_of(const rkv_kv_geometry *g, const rkv_decode_args *a) {
+  Plan pl;
+  pl.unit = 32 * rkv::kMx4Waves;
+  pl.max_len = std::max<int32_t>(a->max_seq_len, 1);
+  const int32_t rows = a->q_len * (a->q_heads / g->kv_heads);
+  pl.target = std::max(1, rkv::kComputeUnits * rkv::mx4_wgs_per_cu(rows, a->q_dtype == RKV_BF16) / g->kv_heads);
+  const int64_t B = std::max<int32_t>(a->batch, 0);
+  const int32_t rounds = (pl.max_len + pl.unit - 1) / pl.unit;
+  pl.kmin = rounds <= kMx4Whole ? rounds : 1;
+  pl.kmax = rounds;
+  if (a->partition_tokens > 0) {
+    pl.pt = a->partition_tokens;
+    pl.n_parts = (pl.max_len + pl.pt - 1) / pl.pt;
+    pl.n_wg = (int32_t)std::min<int64_t>(B * pl.n_parts, INT32_MAX);
+    pl.n_grid = pl.n_wg;
+    pl.direct = pl.n_parts == 1;
+  } else {
+    const int64_t pmin = (int64_t)pl.kmin * pl.unit;
+    pl.n_wg = (int32_t)std::min<int64_t>({std::max<int64_t>(pl.target, B), std::max<int64_t>(B * rounds, 1), INT32_MAX});
+    pl.n_grid = (int32_t)std::min<int64_t>(pl.n_wg, std::max<int64_t>(B * ((pl.max_len + pmin - 1) / pmin), 1));
+    pl.direct = pl.max_len <= pmin;
+  }
+  return pl;
+}
+
 int32_t batch_rows_per_kv(const rkv_kv_geometry *g, const rkv_decode_args *a) {
   return a->q_len * (a->q_heads / g->kv_heads);
 }
@@ -661,7 +700,7 @@ WsLayout ws_layout(const rkv_kv_geometry *g, const rkv_decode_args *a, const Pla
   // (24.8 with partitions of 8 tiles).  72 sequences of about 2000 tokens,
   // 9-tile partitions: 41.2 us with the one slice that this gives, 42.9 with
   // two.
-  const int64_t even = ((int64_t)B * ((pl.max_len + 31) / 32) + pl.target - 1) / pl.target;
+  const int64_t even = ((int64_t)B * ((pl.max_len + pl.unit - 1) / pl.unit) + pl.target - 1) / pl.target;
   const int64_t shortest =
       pl.pt > 0 ? pl.pt : std::max<int64_t>(pl.kmin, std::min<int64_t>(even, 8)) * pl.unit;
   int64_t n_entry = (pl.max_len + shortest - 1) / shortest;
@@ -1133,20 +1172,12 @@ size_t decode_ws_bytes(const rkv_kv_geometry *g, const rkv_decode_args *a, bool 
   return std::max(ws_bytes(g, a, plan_of(g, a, 2, own_scratch)), ws_bytes(g, a, plan_of(g, a, 3, own_scratch)));
 }
 
-// rkv_decode_q8 with an explicit LDS ring depth: 2 (the default, K codes in
-// registers) or 3 (K codes staged in LDS with V, two tiles in flight).
-// own_scratch: see plan_of.
-rkv_status decode_q8(rkv_ctx *ctx, const rkv_kv_geometry *g, const void *pages,
-                     const int32_t *block_tables, int32_t bt_stride, const int32_t *seq_lens,
-                     int32_t n_seqs, const rkv_decode_args *a, void *stream, int32_t stages,
-                     bool own_scratch = false) {
-  const char *op = "rkv_decode_q8";
-  if (rkv_status s = use_device(ctx, op)) return s;
-  if (rkv_status s = check_decode(g, a, op)) return s;
-  if (rkv_status s = check_tables(pages, block_tables, bt_stride, n_seqs, op)) return s;
-  if (!seq_lens) return fail(RKV_ERR_INVALID_ARG, op, "seq_lens is NULL");
-  if (a->batch == 0) return RKV_OK;
-  const Plan pl = plan_of(g, a, stages, own_scratch);
+// The launches of a checked decode: partials through the workspace and their
+// combine, or the rows themselves where one partition covers every sequence.
+rkv_status run_decode(rkv_ctx *ctx, const rkv_kv_geometry *g, const void *pages,
+                      const int32_t *block_tables, int32_t bt_stride, const int32_t *seq_lens,
+                      int32_t n_seqs, const rkv_decode_args *a, void *stream, const Plan &pl,
+                      hipError_t (*launch)(const rkv::DecodeLaunch &, hipStream_t), const char *op) {
   rkv::DecodeLaunch d = make_decode(ctx, g, pages, block_tables, bt_stride, seq_lens, n_seqs, a, pl);
   hipStream_t hs = as_stream(stream);
   if (!pl.direct) {
@@ -1160,7 +1191,7 @@ rkv_status decode_q8(rkv_ctx *ctx, const rkv_kv_geometry *g, const void *pages,
     d.ws_ml = reinterpret_cast<float *>(base + w.ml);
     d.ws_o = reinterpret_cast<float *>(base + w.o);
   }
-  hipError_t e = rkv::launch_decode(d, hs);
+  hipError_t e = launch(d, hs);
   if (e != hipSuccess) return hip_fail(op, e);
   if (!pl.direct) {
     if (a->split_event && (e = hipEventRecord(static_cast<hipEvent_t>(a->split_event), hs)) != hipSuccess)
@@ -1172,6 +1203,23 @@ rkv_status decode_q8(rkv_ctx *ctx, const rkv_kv_geometry *g, const void *pages,
     if ((e = rkv::launch_combine_flat(c, hs)) != hipSuccess) return hip_fail(op, e);
   }
   return RKV_OK;
+}
+
+// rkv_decode_q8 with an explicit LDS ring depth: 2 (the default, K codes in
+// registers) or 3 (K codes staged in LDS with V, two tiles in flight).
+// own_scratch: see plan_of.
+rkv_status decode_q8(rkv_ctx *ctx, const rkv_kv_geometry *g, const void *pages,
+                     const int32_t *block_tables, int32_t bt_stride, const int32_t *seq_lens,
+                     int32_t n_seqs, const rkv_decode_args *a, void *stream, int32_t stages,
+                     bool own_scratch = false) {
+  const char *op = "rkv_decode_q8";
+  if (rkv_status s = use_device(ctx, op)) return s;
+  if (rkv_status s = check_decode(g, a, op)) return s;
+  if (rkv_status s = check_tables(pages, block_tables, bt_stride, n_seqs, op)) return s;
+  if (!seq_lens) return fail(RKV_ERR_INVALID_ARG, op, "seq_lens is NULL");
+  if (a->batch == 0) return RKV_OK;
+  return run_decode(ctx, g, pages, block_tables, bt_stride, seq_lens, n_seqs, a, stream,
+                    plan_of(g, a, stages, own_scratch), rkv::launch_decode, op);
 }
 }  // namespace
 
@@ -1208,6 +1256,33 @@ rkv_status rkv_decode_q8_noalloc(rkv_ctx *ctx, const rkv_kv_geometry *g, const v
   b.workspace_bytes = rkv::kDecodeScratchBytes;
   return decode_q8(ctx, g, pages, block_tables, bt_stride, seq_lens, n_seqs, &b, stream,
                    decode_stages());
+}
+
+size_t rkv_mx4_page_bytes(const rkv_kv_geometry *g) {
+  if (check_mx4_geometry(g, "rkv_mx4_page_bytes") != RKV_OK) return 0;
+  return (size_t)rkv::mx4_page_bytes(to_geo(g));
+}
+
+size_t rkv_decode_mx4_workspace_bytes(const rkv_kv_geometry *g, const rkv_decode_args *a) {
+  if (!a || check_mx4_geometry(g, "rkv_decode_mx4_workspace_bytes") != RKV_OK) return 0;
+  if (a->q_heads < 1 || a->q_heads % g->kv_heads != 0 || a->q_len < 1) return 0;
+  return ws_bytes(g, a, mx4_plan_of(g, a));
+}
+
+rkv_status rkv_decode_mx4(rkv_ctx *ctx, const rkv_kv_geometry *g, const void *pages,
+                          const int32_t *block_tables, int32_t bt_stride, const int32_t *seq_lens,
+                          int32_t n_seqs, const rkv_decode_args *a, void *stream) {
+  const char *op = "rkv_decode_mx4";
+  if (rkv_status s = check_mx4_geometry(g, op)) return s;
+  if (rkv_status s = check_decode(g, a, op)) return s;
+  if (rkv_status s = check_tables(pages, block_tables, bt_stride, n_seqs, op)) return s;
+  if (!seq_lens) return fail(RKV_ERR_INVALID_ARG, op, "seq_lens is NULL");
+  if (a->append)
+    return fail(RKV_ERR_UNSUPPORTED, op, "append: 4-bit rows are appended by rkv_append_mx4 or rkv_append_rope");
+  if (rkv_status s = use_device(ctx, op)) return s;
+  if (a->batch == 0) return RKV_OK;
+  return run_decode(ctx, g, pages, block_tables, bt_stride, seq_lens, n_seqs, a, stream, mx4_plan_of(g, a),
+                    rkv::launch_mx4_decode, op);
 }
 
 rkv_status rkv_decode_q8_partials(rkv_ctx *ctx, const rkv_kv_geometry *g, const void *pages,

@@ -367,6 +367,98 @@ rkv_status rkv_decode_mx4(rkv_ctx *ctx, const rkv_kv_geometry *g, const void *pa
  * partition_tokens 0 it does not fall as batch or max_seq_len grows. */
 size_t rkv_decode_mx4_workspace_bytes(const rkv_kv_geometry *g, const rkv_decode_args *args);
 
+/* ---- norm and position rotation ---------------------------------------------
+ * Query and key rows as a model's projections give them, normed head by head
+ * and rotated by their positions, in one pass:
+ *   x <- x / sqrt(mean(x^2) + eps) * weight           over a head's dims
+ *   (x_i, x_j) <- (x_i cos a - x_j sin a, x_j cos a + x_i sin a)
+ * for every pair p = (i, j) of the first rot_dim dims, with a = freqs[p] times
+ * the row's position on the pair's axis: one axis for text, several (time,
+ * height, width) for images and video.  The reference's model code does both
+ * on the host before its attention ("RMS-norm heads, RoPE",
+ * har/crates/har-demo/src/bin/har-native-qwen3.rs:960-1010).  Angles are
+ * taken in f64: positions of any size keep every bit. */
+typedef struct rkv_rope_args {
+  int32_t rot_dim;          /* dims rotated, a multiple of 8, 0 (none) .. head_dim;
+                               the others pass through the norm only */
+  int32_t adjacent;         /* 0: pairs (i, i + rot_dim/2); 1: (2i, 2i + 1) */
+  const float *freqs;       /* device [rot_dim/2], radians per position */
+  int32_t n_axes;           /* 1..4 */
+  const int32_t *pair_axis; /* device [rot_dim/2]: each pair's axis, 0..n_axes-1 (others
+                               are reported, fault bit 2, and taken as 0); NULL: all 0 */
+  const int32_t *positions; /* device [n_axes][n_rows]; NULL (rkv_append_rope, one
+                               axis): each row's position in its sequence */
+  const void *q_norm;       /* device [head_dim], NULL: queries are not normed */
+  const void *k_norm;       /* device [head_dim], NULL: keys are not normed */
+  int32_t norm_dtype;       /* of both weights: RKV_F32 | RKV_BF16 */
+  float eps;                /* >= 0 */
+} rkv_rope_args;
+
+typedef struct rkv_rope_rows_args {
+  int32_t n_rows;
+  int32_t head_dim;         /* 128 or 256 */
+  int32_t q_heads;          /* 0: no queries */
+  int32_t kv_heads;         /* 0: no keys */
+  const void *q_src;        /* device rows of q_heads * head_dim values ... */
+  const void *k_src;
+  int64_t q_stride;         /* ... q_stride values apart (a packed projection's row
+                               length); 0: dense */
+  int64_t k_stride;
+  int32_t src_dtype;        /* RKV_F32 | RKV_BF16 */
+  void *q_out;              /* device, laid out like the sources; may be the source
+                               itself (same dtype and stride) */
+  void *k_out;
+  int64_t q_out_stride;
+  int64_t k_out_stride;
+  int32_t out_dtype;        /* RKV_F32 | RKV_BF16, rounded once */
+} rkv_rope_rows_args;
+/* Norm and rotation of query and key rows.  Sources, outputs and strides are
+ * multiples of 16 bytes. */
+rkv_status rkv_rope_rows(rkv_ctx *ctx, const rkv_rope_args *rope, const rkv_rope_rows_args *args,
+                         void *stream);
+
+enum { RKV_CACHE_Q8 = 0, RKV_CACHE_MX4 = 1 };  /* page formats */
+typedef struct rkv_append_rope_args {
+  int32_t n_rows;
+  const int32_t *seq_ids;   /* device [n_rows] */
+  const int32_t *positions; /* device [n_rows], token index within the sequence; a
+                               sequence's position appears once in a call */
+  const void *k_src;        /* device rows of kv_heads * head_dim values, k_stride */
+  const void *v_src;        /* and v_stride values apart (0: dense) */
+  int64_t k_stride;
+  int64_t v_stride;
+  int32_t src_dtype;        /* RKV_F32 | RKV_BF16, queries too */
+  int32_t format;           /* RKV_CACHE_Q8 | RKV_CACHE_MX4: what `pages` hold */
+  int32_t rule;             /* Q8: RKV_Q8_CANONICAL | RKV_Q8_HARSERVE; MX4: 0 */
+  const rkv_rope_args *rope;/* NULL: rows are taken as they are */
+  const void *q_src;        /* the same rows' queries, q_heads * head_dim values each,
+                               through the norm and rotation to q_out; NULL: none */
+  int64_t q_stride;
+  int32_t q_heads;
+  void *q_out;              /* device [n_rows][q_heads][head_dim]; may be q_src (dense,
+                               same dtype) */
+  int32_t q_out_dtype;      /* RKV_F32 | RKV_BF16 */
+} rkv_append_rope_args;
+/* Quantize-and-append with the norm and rotation of keys (values go as they
+ * are) on the way, and the rows' queries beside.  Keys are normed and rotated
+ * in f64 and rounded to f32 once; from there a Q8 row has the bytes that
+ * rkv_append_q8 gives it.  With rope NULL and format Q8 it is rkv_append_q8 of
+ * strided rows.  Sources, q_out and strides are multiples of 16 bytes.  Faults
+ * as in rkv_append_q8; their rows are not written (their queries are).  Calls
+ * that overlap must not append to the same 8 tokens (4 with Q8) of a sequence. */
+rkv_status rkv_append_rope(rkv_ctx *ctx, const rkv_kv_geometry *g, void *pages,
+                           const int32_t *block_tables, int32_t bt_stride, int32_t n_seqs,
+                           const rkv_append_rope_args *args, void *stream);
+
+/* The values of cached rows, code times scale (an 8-bit one's in f32): k_out
+ * and v_out [n_rows][kv_heads][head_dim], either may be NULL, 16-byte aligned.
+ * Rows that name no slot are reported as in rkv_append_q8 and read as 0.  (The
+ * reference's q8_0_dequant_row, attention.rs:79-90, a row at a time.) */
+rkv_status rkv_read_rows(rkv_ctx *ctx, const rkv_kv_geometry *g, int32_t format, const void *pages,
+                         const int32_t *block_tables, int32_t bt_stride, int32_t n_seqs,
+                         int32_t n_rows, const int32_t *seq_ids, const int32_t *positions,
+                         void *k_out, void *v_out, int32_t out_dtype, void *stream);
+
 /* Export seq's K or V cache in the reference contiguous layout
  * [kv_heads][len][head_dim/32*34] bytes (what flash_decode_reference reads,
  * attention.rs:144-147; row_to_words is a reinterpretation, :115-120). */

@@ -73,6 +73,30 @@ class DecodeArgs(C.Structure):
                 ("append", C.POINTER(AppendArgs)), ("split_event", P)]
 
 
+class RopeArgs(C.Structure):
+    _fields_ = [("rot_dim", C.c_int32), ("adjacent", C.c_int32), ("freqs", P), ("n_axes", C.c_int32),
+                ("pair_axis", P), ("positions", P), ("q_norm", P), ("k_norm", P),
+                ("norm_dtype", C.c_int32), ("eps", C.c_float)]
+
+
+class RopeRowsArgs(C.Structure):
+    _fields_ = [("n_rows", C.c_int32), ("head_dim", C.c_int32), ("q_heads", C.c_int32),
+                ("kv_heads", C.c_int32), ("q_src", P), ("k_src", P), ("q_stride", C.c_int64),
+                ("k_stride", C.c_int64), ("src_dtype", C.c_int32), ("q_out", P), ("k_out", P),
+                ("q_out_stride", C.c_int64), ("k_out_stride", C.c_int64), ("out_dtype", C.c_int32)]
+
+
+class AppendRopeArgs(C.Structure):
+    _fields_ = [("n_rows", C.c_int32), ("seq_ids", P), ("positions", P), ("k_src", P), ("v_src", P),
+                ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("src_dtype", C.c_int32),
+                ("format", C.c_int32), ("rule", C.c_int32), ("rope", C.POINTER(RopeArgs)),
+                ("q_src", P), ("q_stride", C.c_int64), ("q_heads", C.c_int32), ("q_out", P),
+                ("q_out_dtype", C.c_int32)]
+
+
+CACHE_Q8, CACHE_MX4 = 0, 1
+
+
 class PrefillArgs(C.Structure):
     _fields_ = [("n_seqs", C.c_int32), ("seq_ids", I32P), ("ctx_lens", I32P), ("q_rows", I32P),
                 ("q_offsets", I32P), ("total_rows", C.c_int32), ("q", P), ("q_dtype", C.c_int32),
@@ -167,6 +191,11 @@ _SIGS = {
     "rkv_prefill_workspace_bytes": (C.c_size_t, [C.POINTER(Geometry), C.POINTER(PrefillArgs)]),
     "rkv_pool_prefill_workspace_bytes": (C.c_size_t, [P, C.POINTER(PrefillArgs)]),
     "rkv_decode_partition_tokens": (C.c_int32, [C.POINTER(Geometry), C.POINTER(DecodeArgs)]),
+    "rkv_rope_rows": (C.c_int32, [P, C.POINTER(RopeArgs), C.POINTER(RopeRowsArgs), P]),
+    "rkv_append_rope": (C.c_int32, [P, C.POINTER(Geometry), P, P, C.c_int32, C.c_int32,
+                                    C.POINTER(AppendRopeArgs), P]),
+    "rkv_read_rows": (C.c_int32, [P, C.POINTER(Geometry), C.c_int32, P, P, C.c_int32, C.c_int32,
+                                  C.c_int32, P, P, P, P, C.c_int32, P]),
     "rkv_mx4_page_bytes": (C.c_size_t, [C.POINTER(Geometry)]),
     "rkv_decode_mx4": (C.c_int32, [P, C.POINTER(Geometry), P, P, C.c_int32, P, C.c_int32,
                                    C.POINTER(DecodeArgs), P]),
@@ -595,6 +624,132 @@ def decode_q8_noalloc(ctx: Ctx, g: Geometry, pages, block_tables, seq_lens, a: D
     check(lib().rkv_decode_q8_noalloc(ctx.h, C.byref(g), _ptr(pages), _ptr(block_tables),
                                       block_tables.shape[-1], _ptr(seq_lens), seq_lens.numel(),
                                       C.byref(a), _stream(stream)))
+
+
+def _dtype(t) -> int:
+    """The RKV_* type of a tensor; others are refused here, their bytes would be misread."""
+    import torch
+    if t.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"float32 or bfloat16 wanted, got {t.dtype}")
+    return BF16 if t.dtype == torch.bfloat16 else F32
+
+
+def _i32(t, what: str):
+    import torch
+    if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
+        raise TypeError(f"{what}: a contiguous int32 tensor wanted")
+    return t
+
+
+def _head_rows(t, what: str) -> int:
+    """Row stride of [rows][heads][head_dim] values whose heads lie one after the other."""
+    if t.dim() != 3 or t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+        raise ValueError(f"{what}: [rows][heads][head_dim] with dense heads wanted")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
+def rope_args(rot_dim: int, freqs, positions=None, pair_axis=None, adjacent: bool = False, q_norm=None,
+              k_norm=None, eps: float = 0.0) -> RopeArgs:
+    """freqs [rot_dim/2] f32, positions [rows] or [axes][rows] int32, pair_axis
+    [rot_dim/2] int32, q_norm and k_norm [head_dim] of one type."""
+    import torch
+    n_axes = positions.shape[0] if positions is not None and positions.dim() == 2 else 1
+    if freqs is not None and (freqs.dtype != torch.float32 or not freqs.is_contiguous()):
+        raise TypeError("freqs: a contiguous float32 tensor wanted")
+    if (freqs is not None and freqs.numel() != rot_dim // 2) or \
+            (pair_axis is not None and pair_axis.numel() != rot_dim // 2):
+        raise ValueError("freqs and pair_axis have rot_dim/2 values")
+    norms = [w for w in (q_norm, k_norm) if w is not None]
+    if any(not w.is_contiguous() or w.dtype != norms[0].dtype for w in norms):
+        raise TypeError("q_norm and k_norm: contiguous, of one type")
+    a = RopeArgs(rot_dim, int(adjacent), _ptr(freqs), n_axes, _ptr(_i32(pair_axis, "pair_axis")),
+                 _ptr(_i32(positions, "positions")), _ptr(q_norm), _ptr(k_norm),
+                 _dtype(norms[0]) if norms else F32, eps)
+    a._refs = (freqs, positions, pair_axis, q_norm, k_norm)
+    a._rows = None if positions is None else positions.shape[-1]
+    return a
+
+
+def _rope_fits(rope, n_rows: int, *heads) -> None:
+    if rope is None:
+        return
+    if rope._rows is not None and rope._rows != n_rows:
+        raise ValueError(f"{rope._rows} rope positions for {n_rows} rows")
+    for w, t in heads:
+        if w is not None and t is not None and w.numel() != t.shape[2]:
+            raise ValueError("a norm weight has head_dim values")
+
+
+def rope_rows(ctx: Ctx, rope: RopeArgs, q, k, q_out, k_out, stream=None) -> None:
+    """Norm and rotation of q and k [rows][heads][head_dim] (views with any row
+    stride; either may be None) into q_out and k_out of the same shapes."""
+    one = q if q is not None else k
+    n, D = one.shape[0], one.shape[2]
+    for t, o in ((q, q_out), (k, k_out)):
+        if t is not None and (t.shape != o.shape or t.shape[0] != n or t.shape[2] != D or t.dtype != one.dtype):
+            raise ValueError("q, k and their outputs: one number of rows, head_dim and type, shapes alike")
+    outs = [o for t, o in ((q, q_out), (k, k_out)) if t is not None]
+    if any(o.dtype != outs[0].dtype for o in outs):
+        raise ValueError("q_out and k_out have one type")
+    _rope_fits(rope, n, (rope._refs[3], q), (rope._refs[4], k))
+    a = RopeRowsArgs(n, D, q.shape[1] if q is not None else 0, k.shape[1] if k is not None else 0,
+                     _ptr(q), _ptr(k), _head_rows(q, "q") if q is not None else 0,
+                     _head_rows(k, "k") if k is not None else 0, _dtype(one),
+                     _ptr(q_out) if q is not None else None, _ptr(k_out) if k is not None else None,
+                     _head_rows(q_out, "q_out") if q is not None else 0,
+                     _head_rows(k_out, "k_out") if k is not None else 0, _dtype(outs[0]))
+    check(lib().rkv_rope_rows(ctx.h, C.byref(rope), C.byref(a), _stream(stream)))
+
+
+def append_rope_args(fmt: int, seq_ids, positions, k_src, v_src, rope: RopeArgs | None = None, q=None,
+                     q_out=None, rule: int = Q8_CANONICAL) -> AppendRopeArgs:
+    """Rows [n][kv_heads][head_dim] (views with any row stride) of one append;
+    q [n][q_heads][head_dim] goes normed and rotated to q_out (contiguous)."""
+    n = seq_ids.numel()
+    for t in (k_src, v_src, q):
+        if t is not None and (t.shape[0] != n or t.shape[2] != k_src.shape[2] or t.dtype != k_src.dtype):
+            raise ValueError("k, v and q: one number of rows, head_dim and type")
+    if v_src.shape != k_src.shape or positions.numel() != n:
+        raise ValueError("v and positions go with k")
+    if q is not None and (q_out.shape != q.shape or not q_out.is_contiguous()):
+        raise ValueError("q_out: contiguous, shaped like q")
+    if rope is not None:
+        _rope_fits(rope, n, (rope._refs[3], q), (rope._refs[4], k_src))
+    a = AppendRopeArgs(n, _ptr(_i32(seq_ids, "seq_ids")), _ptr(_i32(positions, "positions")), _ptr(k_src), _ptr(v_src),
+                       _head_rows(k_src, "k"), _head_rows(v_src, "v"), _dtype(k_src), fmt, rule,
+                       C.pointer(rope) if rope is not None else None, _ptr(q),
+                       _head_rows(q, "q") if q is not None else 0, q.shape[1] if q is not None else 0,
+                       _ptr(q_out) if q is not None else None, _dtype(q_out) if q is not None else F32)
+    a._refs = (seq_ids, positions, k_src, v_src, rope, q, q_out)
+    a._heads = k_src.shape[1:]
+    return a
+
+
+def append_rope(ctx: Ctx, g: Geometry, fmt: int, pages, block_tables, seq_ids, positions, k_src, v_src,
+                rope: RopeArgs | None = None, q=None, q_out=None, rule: int = Q8_CANONICAL, stream=None) -> None:
+    """Quantize-and-append into pages of format CACHE_Q8 or CACHE_MX4, keys
+    normed and rotated on the way (rope), the rows' queries beside."""
+    a = append_rope_args(fmt, seq_ids, positions, k_src, v_src, rope, q, q_out, rule)
+    if tuple(a._heads) != (g.kv_heads, g.head_dim):
+        raise ValueError("k and v rows have the geometry's heads")
+    check(lib().rkv_append_rope(ctx.h, C.byref(g), _ptr(pages), _ptr(block_tables), block_tables.shape[-1],
+                                block_tables.shape[0], C.byref(a), _stream(stream)))
+
+
+def read_rows(ctx: Ctx, g: Geometry, fmt: int, pages, block_tables, seq_ids, positions, k_out, v_out,
+              stream=None) -> None:
+    """Values of cached rows into k_out, v_out [n][kv_heads][head_dim] (either may be None)."""
+    n = seq_ids.numel()
+    for t in (k_out, v_out):
+        if t is not None and (tuple(t.shape) != (n, g.kv_heads, g.head_dim) or not t.is_contiguous()):
+            raise ValueError("outputs: contiguous [rows][kv_heads][head_dim]")
+    outs = [t for t in (k_out, v_out) if t is not None]
+    if positions.numel() != n or any(t.dtype != outs[0].dtype for t in outs):
+        raise ValueError("one position a row, outputs of one type")
+    check(lib().rkv_read_rows(ctx.h, C.byref(g), fmt, _ptr(pages), _ptr(block_tables), block_tables.shape[-1],
+                              block_tables.shape[0], n, _ptr(_i32(seq_ids, "seq_ids")),
+                              _ptr(_i32(positions, "positions")), _ptr(k_out), _ptr(v_out),
+                              _dtype(outs[0]) if outs else F32, _stream(stream)))
 
 
 def mx4_page_bytes(g: Geometry) -> int:

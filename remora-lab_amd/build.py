@@ -15,7 +15,7 @@ CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "librkv.so")
 OBJDIR = os.path.join(HERE, "_build")
 
-SOURCES = ["rkv_append.hip", "rkv_decode.hip", "rkv_decode_rows32.hip", "rkv_mx4_decode.hip",
+SOURCES = ["rkv_append.hip", "rkv_decode.hip", "rkv_decode_rows32.hip", "rkv_mx4_decode.hip", "rkv_rope.hip",
            "rkv_prefill.hip",
            "rkv_r4kv.hip", "rkv_stream.hip", "rkv_scratch.hip", "rkv_runtime.cpp", "rkv_serve.cpp"]
 

@@ -26,6 +26,51 @@ struct AppendLaunch {
 };
 hipError_t launch_append(const AppendLaunch &a, hipStream_t s);
 
+// Per-head norm and position rotation of a call's rows (rkv_rope_args).
+struct RopeLaunch {
+  int32_t on;        // 0: rows pass as they are
+  int32_t rot_dim;   // leading dims rotated, a multiple of 8
+  int32_t adjacent;  // pairs (2i, 2i+1), else (i, i + rot_dim/2)
+  int32_t n_axes;
+  const float *freqs;
+  const int32_t *pair_axis;  // nullptr: axis 0
+  const int32_t *positions;  // [n_axes][n_rows]; nullptr: the appended positions
+  const void *q_norm, *k_norm;
+  int32_t norm_bf16;
+  float eps;
+  int32_t n_rows;
+  int32_t *fault;
+};
+// Rows of heads in and out, strides in elements between rows.
+struct HeadRows {
+  const void *src;
+  void *out;
+  int64_t stride, out_stride;
+  int32_t heads;
+  int32_t bf16, out_bf16;
+};
+hipError_t launch_rope_rows(const RopeLaunch &r, const HeadRows &q, const HeadRows &k, int32_t head_dim,
+                            hipStream_t s);
+// Append through the rotation into Q8_0 (mx4 0) or 4-bit (1) pages, and the
+// queries q of the same rows (q.src nullptr: none).
+struct AppendRopeLaunch {
+  AppendLaunch a;
+  int64_t k_stride, v_stride;
+  int32_t mx4;
+  RopeLaunch r;
+  HeadRows q;
+};
+hipError_t launch_append_rope(const AppendRopeLaunch &a, hipStream_t s);
+// Values of cached rows: k_out, v_out [n_rows][kv_heads][head_dim] (a.a's
+// pages, tables, rows); rows that name no slot are reported and read as 0.
+struct ReadRowsLaunch {
+  AppendLaunch a;
+  int32_t mx4;
+  void *k_out, *v_out;
+  int32_t out_bf16;
+};
+hipError_t launch_read_rows(const ReadRowsLaunch &a, hipStream_t s);
+
 // gather: pages -> reference rows; import: reference rows -> pages
 hipError_t launch_gather(const Geo &g, const uint8_t *pages, const int32_t *bt, int32_t len,
                          int32_t kind, uint8_t *rows, int32_t *fault, hipStream_t s);

@@ -1,0 +1,669 @@
+// rkv_rope.hip -- per-head norm and position rotation of query and key rows,
+// the same on the way into the paged cache (Q8_0 or 4-bit pages), and cached
+// rows read back as values (gfx950).
+//
+//   n = x / sqrt(mean(x^2) + eps) * w            (head by head, if a weight is given)
+//   a_i = position[axis_i] * freq_i              (pair i of the rotated dims)
+//   (x_i, x_j) -> (x_i cos a_i - x_j sin a_i, x_j cos a_i + x_i sin a_i)
+//
+// Angles are exact in f64 (24 + 31 bits) and reduced there, so a position of a
+// million keeps every bit.  A key on its way into the cache is normed and
+// rotated in f64 and rounded to f32 once, before the quantizer: f64 runs at
+// the f32 rate here, and a page byte then follows from the definition alone,
+// not from an order of sums (an f32 rotation moves about one code in 10^6 over
+// a border).  Rows that are returned go in f32.
+//
+// A head is held by D/8 lanes, 8 values each: lane c of a rotated pair of
+// halves takes dims 4c..4c+3 and rot/2 + 4c.., so both values of its 4 pairs
+// are its own and their cosines serve every head of the row.
+#include <algorithm>
+
+#include "rkv_launch.h"
+#include "rkv_mx4.h"
+
+namespace rkv {
+namespace {
+
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+
+#if defined(__HIP_DEVICE_COMPILE__)
+
+// ---- angles -------------------------------------------------------------------
+
+// sin and cos of a by their Taylor series on [-pi/4, pi/4], whose first terms
+// left out are below 5e-17.  Reduction: a - n*pi/2 with pi/2 in two parts, each
+// step one fma, for |a| up to 2^31 and more.
+__device__ __forceinline__ void sin_cos(double a, double &s, double &c) {
+  const double n = __builtin_rint(a * 0.63661977236758134308);
+  double r = __builtin_fma(-n, 0x1.921fb54442d18p+0, a);
+  r = __builtin_fma(-n, 0x1.1a62633145c07p-54, r);
+  const double z = r * r;
+  double ps = -1.0 / 1307674368000.0;  // 15!
+  ps = __builtin_fma(ps, z, 1.0 / 6227020800.0);
+  ps = __builtin_fma(ps, z, -1.0 / 39916800.0);
+  ps = __builtin_fma(ps, z, 1.0 / 362880.0);
+  ps = __builtin_fma(ps, z, -1.0 / 5040.0);
+  ps = __builtin_fma(ps, z, 1.0 / 120.0);
+  ps = __builtin_fma(ps, z, -1.0 / 6.0);
+  ps = __builtin_fma(r * z, ps, r);
+  double pc = 1.0 / 20922789888000.0;  // 16!
+  pc = __builtin_fma(pc, z, -1.0 / 87178291200.0);
+  pc = __builtin_fma(pc, z, 1.0 / 479001600.0);
+  pc = __builtin_fma(pc, z, -1.0 / 3628800.0);
+  pc = __builtin_fma(pc, z, 1.0 / 40320.0);
+  pc = __builtin_fma(pc, z, -1.0 / 720.0);
+  pc = __builtin_fma(pc, z, 1.0 / 24.0);
+  pc = __builtin_fma(pc, z, -0.5);
+  pc = __builtin_fma(pc, z, 1.0);
+  const int q = (int)(n - 4.0 * __builtin_floor(n * 0.25));  // quadrant
+  s = q & 1 ? pc : ps;
+  c = q & 1 ? ps : pc;
+  s = q & 2 ? -s : s;
+  c = (q + 1) & 2 ? -c : c;
+}
+
+// Cosines and sines of lane c's 4 pairs of a row (1 and 0 past the rotated dims).
+struct Turn {
+  double c[4], s[4];
+  __device__ __forceinline__ void load(const RopeLaunch &r, int64_t row, int32_t pos, int lane) {
+    const bool in = 8 * lane < r.rot_dim;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      c[i] = 1.0;
+      s[i] = 0.0;
+      if (!in) continue;
+      const int pair = 4 * lane + i;
+      int32_t axis = r.pair_axis != nullptr ? r.pair_axis[pair] : 0;
+      if (axis < 0 || axis >= r.n_axes) {
+        atomicOr(r.fault, FAULT_BAD_POSITION);
+        axis = 0;
+      }
+      const int32_t p = r.positions != nullptr ? r.positions[(int64_t)axis * r.n_rows + row] : pos;
+      sin_cos((double)p * (double)r.freqs[pair], s[i], c[i]);
+    }
+  }
+};
+
+// ---- sums over a head's lanes ----------------------------------------------------
+
+template <int kCtrl>
+__device__ __forceinline__ float dpp(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), kCtrl, 0xf, 0xf, false));
+}
+template <int kCtrl>
+__device__ __forceinline__ double dpp(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, kCtrl, 0xf, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), kCtrl, 0xf, 0xf, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// Over kLanes (16 or 32) consecutive lanes: swaps within quads, halves of a
+// row and the row, then the neighbouring row.
+template <int kLanes, typename T>
+__device__ __forceinline__ T lanes_sum(T x) {
+  x += dpp<0xb1>(x);   // quad_perm 1 0 3 2
+  x += dpp<0x4e>(x);   // quad_perm 2 3 0 1
+  x += dpp<0x141>(x);  // row_half_mirror
+  x += dpp<0x140>(x);  // row_mirror
+  if constexpr (kLanes == 32) x += __shfl_xor(x, 16);
+  return x;
+}
+
+__device__ __forceinline__ float inv_sqrt(float x) { return __builtin_amdgcn_rsqf(x); }
+__device__ __forceinline__ double inv_sqrt(double x) {
+  double y = __builtin_amdgcn_rsq(x);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) y = __builtin_fma(y * __builtin_fma(-x * y, y, 1.0), 0.5, y);
+  return x == __builtin_inf() ? 0.0 : y;
+}
+
+// ---- one head ------------------------------------------------------------------
+
+// The dims of lane c: 4 from first(), 4 from second().
+struct Dims {
+  int a, b;
+  __device__ __forceinline__ Dims(const RopeLaunch &r, int c) {
+    const bool halves = r.on && !r.adjacent && 8 * c < r.rot_dim;
+    a = halves ? 4 * c : 8 * c;
+    b = halves ? r.rot_dim / 2 + 4 * c : 8 * c + 4;
+  }
+};
+
+__device__ __forceinline__ void load4(const void *src, int64_t at, bool bf16, float (&v)[8], int to) {
+  if (bf16) {
+    const v2u w = *reinterpret_cast<const v2u *>(static_cast<const uint16_t *>(src) + at);
+    v[to] = __builtin_bit_cast(float, w[0] << 16);
+    v[to + 1] = __builtin_bit_cast(float, w[0] & 0xffff0000u);
+    v[to + 2] = __builtin_bit_cast(float, w[1] << 16);
+    v[to + 3] = __builtin_bit_cast(float, w[1] & 0xffff0000u);
+  } else {
+    const v4f w = *reinterpret_cast<const v4f *>(static_cast<const float *>(src) + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[to + i] = w[i];
+  }
+}
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  return (uint32_t)f32_to_bf16_rtne(a) | (uint32_t)f32_to_bf16_rtne(b) << 16;
+}
+__device__ __forceinline__ void store4(void *out, int64_t at, bool bf16, const float (&v)[8], int from) {
+  if (bf16)
+    *reinterpret_cast<v2u *>(static_cast<uint16_t *>(out) + at) =
+        v2u{pack_bf16(v[from], v[from + 1]), pack_bf16(v[from + 2], v[from + 3])};
+  else
+    *reinterpret_cast<v4f *>(static_cast<float *>(out) + at) = v4f{v[from], v[from + 1], v[from + 2], v[from + 3]};
+}
+
+// A norm weight's values at a lane's dims.
+__device__ __forceinline__ void load_weight(const void *w, bool bf16, const Dims &d, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int at = i < 4 ? d.a + i : d.b + i - 4;
+    v[i] = w == nullptr ? 1.0f
+           : bf16       ? bf16_bits_to_f32(static_cast<const uint16_t *>(w)[at])
+                        : static_cast<const float *>(w)[at];
+  }
+}
+
+// Norm and rotation of a head's 8 values in this lane, in T.
+template <typename T, int D>
+__device__ __forceinline__ void turn_head(float (&v)[8], const RopeLaunch &r, bool norm, const float (&w)[8],
+                                          const Turn &t, bool rotated) {
+  T x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = (T)v[i];
+  if (norm) {
+    T q = x[0] * x[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) q = __builtin_elementwise_fma(x[i], x[i], q);
+    const T f = inv_sqrt(lanes_sum<D / 8>(q) * (T)(1.0 / D) + (T)r.eps);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] *= f * (T)w[i];
+  }
+  if (rotated) {
+    T y[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int a = r.adjacent ? 2 * i : i, b = r.adjacent ? 2 * i + 1 : i + 4;
+      const T c = (T)t.c[i], s = (T)t.s[i];
+      y[a] = __builtin_elementwise_fma(x[a], c, -(x[b] * s));
+      y[b] = __builtin_elementwise_fma(x[b], c, x[a] * s);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = y[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = (float)x[i];
+}
+
+// Heads [h0, h1) of one row, by one wave, 512/D at a time.
+template <int D>
+__device__ __forceinline__ void turn_row(const RopeLaunch &r, const HeadRows &m, const void *weight, int64_t row,
+                                         int32_t pos, int h0, int h1, int lane) {
+  constexpr int L = D / 8, kHeads = 64 / L;
+  const int c = lane % L;
+  const Dims d(r, c);
+  const bool rotated = 8 * c < r.rot_dim;
+  float w[8];
+  load_weight(weight, r.norm_bf16 != 0, d, w);
+  float v[8] = {};
+  const int64_t src = row * m.stride, dst = row * m.out_stride;
+  int h = h0 + lane / L;
+  if (h < h1) {
+    load4(m.src, src + (int64_t)h * D + d.a, m.bf16 != 0, v, 0);
+    load4(m.src, src + (int64_t)h * D + d.b, m.bf16 != 0, v, 4);
+  }
+  Turn t;
+  t.load(r, row, pos, c);
+  for (int b = h0; b < h1; b += kHeads, h += kHeads) {
+    float n[8] = {};
+    if (h + kHeads < h1) {
+      load4(m.src, src + (int64_t)(h + kHeads) * D + d.a, m.bf16 != 0, n, 0);
+      load4(m.src, src + (int64_t)(h + kHeads) * D + d.b, m.bf16 != 0, n, 4);
+    }
+    turn_head<float, D>(v, r, weight != nullptr, w, t, rotated);
+    if (h < h1) {
+      store4(m.out, dst + (int64_t)h * D + d.a, m.out_bf16 != 0, v, 0);
+      store4(m.out, dst + (int64_t)h * D + d.b, m.out_bf16 != 0, v, 4);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = n[i];
+  }
+}
+#endif  // __HIP_DEVICE_COMPILE__
+
+// Wave x takes head chunk x % (nq + nk) of row x / (nq + nk): nq chunks of
+// `chunk` query heads, then nk of key heads.
+template <int D>
+__global__ __launch_bounds__(256) void rope_rows_kernel(RopeLaunch r, HeadRows q, HeadRows k, int32_t chunk) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const int lane = threadIdx.x & 63;
+  const int nq = (q.heads + chunk - 1) / chunk, nk = (k.heads + chunk - 1) / chunk;
+  const int64_t x = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row = x / (nq + nk);
+  const int at = (int)(x % (nq + nk));
+  if (row >= r.n_rows) return;
+  if (at < nq) turn_row<D>(r, q, r.q_norm, row, 0, at * chunk, min(q.heads, (at + 1) * chunk), lane);
+  else turn_row<D>(r, k, r.k_norm, row, 0, (at - nq) * chunk, min(k.heads, (at - nq + 1) * chunk), lane);
+#endif
+}
+
+// ---- append ------------------------------------------------------------------------
+#if defined(__HIP_DEVICE_COMPILE__)
+
+// E2M1 codes of this lane's 8 values of a block held by 4 consecutive lanes,
+// and the block's exponent (999: not finite).
+template <int kKind>
+__device__ __forceinline__ uint32_t mx4_quantize8(const float (&v)[8], int32_t &e) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, __builtin_bit_cast(uint32_t, v[i]) & 0x7fffffffu);
+  top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xb1, 0xf, 0xf, false));
+  top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4e, 0xf, 0xf, false));
+  // |v| = m * 2^x, m in [1, 2): at most 7 * 2^(x-2) up to m = 1.75
+  e = (int32_t)(top >> 23) - 127 - ((top & 0x7fffffu) <= 0x600000u ? 2 : 1);
+  e = min(max(e, kKind == 0 ? kMx4KMin : kMx4VMin), kKind == 0 ? kMx4KMax : kMx4VMax);
+  const float scale = __builtin_bit_cast(float, (uint32_t)(e + 127) << 23);
+  uint32_t w = 0;
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0], v[1], scale, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2], v[3], scale, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4], v[5], scale, 2);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6], v[7], scale, 3);
+  if (top >= 0x7f800000u) {
+    e = 999;
+    w = 0;
+  }
+  return w;
+}
+
+// The low nibbles of 8 bytes, byte k to nibble k.
+__device__ __forceinline__ uint32_t low_nibbles(uint32_t w0, uint32_t w1) {
+  w0 &= 0x0f0f0f0fu;
+  w1 &= 0x0f0f0f0fu;
+  w0 = (w0 | w0 >> 4) & 0x00ff00ffu;
+  w1 = (w1 | w1 >> 4) & 0x00ff00ffu;
+  return ((w0 | w0 >> 8) & 0xffffu) | (w1 | w1 >> 8) << 16;
+}
+#endif  // __HIP_DEVICE_COMPILE__
+
+// Workgroup x of the first append_blocks takes input rows [ROWS*(x / groups),
+// +ROWS) and kv heads [heads*(x % groups), +heads); the others are the query
+// waves (rope_rows_kernel's, keys none).
+//  1. wave 0 finds each row's page and slot; rows that have none are reported
+//     and skipped.
+//  2. K: 512/D rows a wave, normed and rotated in f64, through LDS into 8
+//     consecutive dims a lane, quantized by 4 lanes a block and stored.
+//  3. V: codes of tokens that are neighbours share words of a page (4 tokens
+//     of a Q8_0 tile's dim, 8 of a 4-bit one's).  A run is the rows that
+//     follow each other inside one such group of slots; the workgroup that
+//     holds its first row takes all of it (rows past its own among them), puts
+//     the codes through LDS and stores whole words.  A run that does not fill
+//     its group leaves the other tokens' bits alone: bytes, and in 4-bit pages
+//     an atomic xor of the words' own bits (another run of the call may hold
+//     the rest of the word).
+template <int D, bool kMx4, int ROWS, bool kBf16>
+__global__ __launch_bounds__(256) void append_rope_kernel(AppendRopeLaunch p, int32_t groups, int32_t heads,
+                                                          uint32_t append_blocks, int32_t chunk) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr int L = D / 8, RW = 64 / L, NB = D / 32;
+  constexpr int GROUP = kMx4 ? 8 : 4;        // tokens of a V word
+  constexpr int VR = ROWS + GROUP - 1;       // V rows a workgroup may take
+  constexpr int CB = kMx4 ? D / 2 : D;       // code bytes of a row
+  constexpr int CS = CB + 8;                 // LDS row stride
+  __shared__ __attribute__((aligned(16))) float turned[4][RW][D];
+  __shared__ __attribute__((aligned(16))) uint8_t codes[VR][CS];
+  __shared__ uint16_t scales[VR][NB];
+  __shared__ int64_t rbase[VR + 1];  // the row's page, bytes into the pool; -1: skip
+  __shared__ int32_t rslot[VR + 1], rpos[VR + 1];
+  __shared__ uint64_t starts;        // rows that start a run
+  __shared__ int32_t vend;           // end of the rows that this workgroup's runs take
+  const AppendLaunch &a = p.a;
+  const Geo g = a.g;
+  const int tid = (int)threadIdx.x, lane = tid & 63;
+  const int wave = (int)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (blockIdx.x >= append_blocks) {
+    const int nq = (p.q.heads + chunk - 1) / chunk;
+    const int64_t x = (int64_t)(blockIdx.x - append_blocks) * 4 + wave;
+    const int64_t row = x / nq;
+    const int at = (int)(x % nq);
+    if (row < a.n_rows)
+      turn_row<D>(p.r, p.q, p.r.q_norm, row, a.positions[row], at * chunk, min(p.q.heads, (at + 1) * chunk), lane);
+    return;
+  }
+  const int64_t row0 = (int64_t)(blockIdx.x / groups) * ROWS;
+  const int h0 = (int)(blockIdx.x % groups) * heads, h1 = min(g.kv_heads, h0 + heads);
+  const int nr = (int)min<int64_t>(ROWS, (int64_t)a.n_rows - row0);
+  const uint64_t PB = kMx4 ? mx4_page_bytes(g) : page_bytes(g);
+  const uint64_t RB = kMx4 ? mx4_region_bytes(g) : region_bytes(g);
+
+  if (wave == 0) {
+    const bool in = lane <= VR && row0 + lane < a.n_rows;
+    int32_t seq = -1, pos = -1;
+    if (in) {
+      seq = a.seq_ids[row0 + lane];
+      pos = a.positions[row0 + lane];
+    }
+    int32_t pseq = __shfl_up(seq, 1), ppos = __shfl_up(pos, 1);
+    if (lane == 0 && row0 > 0) {
+      pseq = a.seq_ids[row0 - 1];
+      ppos = a.positions[row0 - 1];
+    }
+    int64_t base = -1;
+    int32_t bad = 0;
+    if (in) {
+      if (seq < 0 || seq >= a.n_seqs) bad = FAULT_BAD_SEQ;
+      else if (pos < 0 || pos / g.page_tokens >= a.bt_stride) bad = FAULT_BAD_POSITION;
+      else {
+        const int32_t page = a.bt[(int64_t)seq * a.bt_stride + pos / g.page_tokens];
+        if (page < 0 || page >= g.num_pages) bad = FAULT_BAD_PAGE;
+        else base = (int64_t)((uint64_t)page * PB);
+      }
+      if (bad != 0 && h0 == 0 && lane < nr) atomicOr(a.fault, bad);
+    }
+    const bool follows = (lane > 0 || row0 > 0) && seq == pseq && pos == ppos + 1 && pos % GROUP != 0;
+    const uint64_t s = __ballot(in && !follows);
+    if (lane <= VR) {
+      rbase[lane] = base;
+      rslot[lane] = pos % g.page_tokens;
+      rpos[lane] = pos;
+    }
+    if (lane == 0) {
+      const int avail = (int)min<int64_t>(VR, (int64_t)a.n_rows - row0);
+      const uint64_t mine = s & ((1ull << nr) - 1ull), later = s & ~((1ull << nr) - 1ull);
+      starts = mine;
+      vend = mine == 0 ? 0 : later == 0 ? avail : min(avail, (int)__builtin_ctzll(later));
+    }
+  }
+  __syncthreads();
+
+  const int c = lane % L, sub = lane / L;
+  // ---- K ----------------------------------------------------------------------
+  const Dims d(p.r, c);
+  const bool rotated = p.r.on && 8 * c < p.r.rot_dim;
+  float w[8];
+  load_weight(p.r.on ? p.r.k_norm : nullptr, p.r.norm_bf16 != 0, d, w);
+  for (int i = RW * wave; i < nr; i += 4 * RW) {
+    const int r = min(i + sub, nr - 1);
+    const bool live = i + sub < nr && rbase[r] >= 0;
+    Turn t;
+    if (p.r.on) t.load(p.r, row0 + r, rpos[r], c);
+    for (int h = h0; h < h1; ++h) {
+      float v[8];
+      const int64_t at = (row0 + r) * p.k_stride + (int64_t)h * D;
+      load4(a.k_src, at + d.a, kBf16, v, 0);
+      load4(a.k_src, at + d.b, kBf16, v, 4);
+      if (p.r.on) turn_head<double, D>(v, p.r, p.r.k_norm != nullptr, w, t, rotated);
+      // to 8 consecutive dims a lane, within the wave
+      float *row = turned[wave][sub];
+      *reinterpret_cast<v4f *>(row + d.a) = v4f{v[0], v[1], v[2], v[3]};
+      *reinterpret_cast<v4f *>(row + d.b) = v4f{v[4], v[5], v[6], v[7]};
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      const v4f x0 = *reinterpret_cast<const v4f *>(row + 8 * c), x1 = *reinterpret_cast<const v4f *>(row + 8 * c + 4);
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        v[k] = x0[k];
+        v[4 + k] = x1[k];
+      }
+      const int blk = c / 4;
+      uint8_t *region = a.pages + (live ? rbase[r] : 0) + (uint64_t)(2 * h) * RB;
+      const int slot = rslot[r];
+      if constexpr (kMx4) {
+        int32_t e;
+        const uint32_t q = mx4_quantize8<0>(v, e);
+        if (live) {
+          uint8_t *tile = region + (uint64_t)(slot / 32) * mx4_tile_bytes(D);
+          const int tok = slot % 32, j = tok % 8 / 4, m = 4 * (tok / 8) + tok % 4, jh = j * (D / 128) + blk / 4;
+          *reinterpret_cast<uint32_t *>(tile + (jh * 4 + blk % 4) * 256 + m * 16 + 4 * (c % 4)) = q;
+          if (c % 4 == 0) tile[16 * D + (blk % 4 * 16 + m) * (D / 64) + jh] = e == 999 ? 255 : (uint8_t)(e + 127);
+        }
+      } else {
+        uint16_t scale;
+        const uint64_t q = q8_quantize_values<8>(v, a.rule, scale);
+        if (live) {
+          *reinterpret_cast<uint64_t *>(region + (uint64_t)slot * D + 8 * c) = q;
+          if (c % 4 == 0) *reinterpret_cast<uint16_t *>(region + scale_offset(g, slot, blk)) = scale;
+        }
+      }
+    }
+  }
+
+  // ---- V ----------------------------------------------------------------------
+  const uint64_t runs = starts;
+  const int v0 = runs != 0 ? (int)__builtin_ctzll(runs) : 0, v1 = vend;
+  for (int h = h0; h < h1; ++h) {
+    if (h > h0) __syncthreads();
+    for (int i = v0 + RW * wave; i < v1; i += 4 * RW) {
+      const int r = min(i + sub, v1 - 1);
+      float v[8];
+      const int64_t at = (row0 + r) * p.v_stride + (int64_t)h * D + 8 * c;
+      load4(a.v_src, at, kBf16, v, 0);
+      load4(a.v_src, at + 4, kBf16, v, 4);
+      if constexpr (kMx4) {
+        int32_t e;
+        const uint32_t q = mx4_quantize8<1>(v, e);
+        *reinterpret_cast<uint32_t *>(&codes[r][4 * c]) = q;
+        if (c % 4 == 0) scales[r][c / 4] = e == 999 ? 0x7e : (uint16_t)(4 * (e + 23));
+      } else {
+        uint16_t scale;
+        const uint64_t q = q8_quantize_values<8>(v, a.rule, scale);
+        *reinterpret_cast<uint64_t *>(&codes[r][8 * c]) = q ^ 0x8080808080808080ull;  // stored biased (code_bias)
+        if (c % 4 == 0) scales[r][c / 4] = scale;
+      }
+    }
+    __syncthreads();
+    // run by run, each by one wave
+    int at = 0;
+    for (uint64_t left = runs; left != 0; left &= left - 1, ++at) {
+      if (at % 4 != wave) continue;
+      const int r = (int)__builtin_ctzll(left);
+      const uint64_t next = left & (left - 1);
+      const int n = (next != 0 ? (int)__builtin_ctzll(next) : v1) - r;  // 1..GROUP rows
+      const int64_t base = rbase[r];
+      if (base < 0) continue;
+      const int slot = rslot[r], first = slot % GROUP;
+      uint8_t *region = a.pages + base + (uint64_t)(2 * h + 1) * RB;
+      if constexpr (kMx4) {
+        uint8_t *tile = region + (uint64_t)(slot / 32) * mx4_tile_bytes(D);
+        const int grp = slot % 32 / 8;
+        if (lane < D / 4) {  // (c, n): 4 words, of the even and odd dims 2n of blocks 2c and 2c + 1
+          const int cc = lane / 16, nn = lane % 16;
+          uint32_t b[2][2] = {{0, 0}, {0, 0}};
+          for (int k = 0; k < n; ++k) {
+            const int t = first + k;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) b[u][t / 4] |= (uint32_t)codes[r + k][32 * cc + 16 * u + nn] << (8 * (t % 4));
+          }
+          v4u q = {low_nibbles(b[0][0], b[0][1]), low_nibbles(b[0][0] >> 4, b[0][1] >> 4),
+                   low_nibbles(b[1][0], b[1][1]), low_nibbles(b[1][0] >> 4, b[1][1] >> 4)};
+          uint32_t *dst = reinterpret_cast<uint32_t *>(tile + cc * 1024 + (grp * 16 + nn) * 16);
+          if (n == 8) {
+            *reinterpret_cast<v4u *>(dst) = q;
+          } else {
+            const uint32_t own = ((1u << (4 * n)) - 1u) << (4 * first);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t was = __hip_atomic_load(dst + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+              const uint32_t flip = (was ^ q[k]) & own;
+              if (flip != 0) atomicXor(dst + k, flip);
+            }
+          }
+        }
+        if (lane < NB * 8) {
+          const int blk = lane / 8, k = lane % 8 - first;
+          if (k >= 0 && k < n) tile[16 * D + (grp * NB + blk) * 8 + lane % 8] = (uint8_t)scales[r + k][blk];
+        }
+      } else {
+        for (int x = lane; x < D; x += 64) {
+          uint8_t *dst = region + code_offset(g, 1, slot, x);
+          if (n == 4) {
+            *reinterpret_cast<uint32_t *>(dst) = (uint32_t)codes[r][x] | (uint32_t)codes[r + 1][x] << 8 |
+                                                 (uint32_t)codes[r + 2][x] << 16 | (uint32_t)codes[r + 3][x] << 24;
+          } else {
+            for (int k = 0; k < n; ++k) dst[k] = codes[r + k][x];
+          }
+        }
+        if (lane < NB * 4) {
+          const int blk = lane / 4, k = lane % 4;
+          if (k < n)
+            *reinterpret_cast<uint16_t *>(region + scale_offset(g, slot + k, blk)) = scales[r + k][blk];
+        }
+      }
+    }
+  }
+#endif  // __HIP_DEVICE_COMPILE__
+}
+
+// ---- rows read back -----------------------------------------------------------------
+
+// One thread per 8 consecutive dims of (row, kv head, kind).
+template <int D, bool kMx4>
+__global__ __launch_bounds__(256) void read_rows_kernel(ReadRowsLaunch p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr int L = D / 8;
+  const AppendLaunch &a = p.a;
+  const Geo g = a.g;
+  const int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int c = (int)(x % L);
+  const int kind = (int)(x / L % 2);
+  const int h = (int)(x / (2 * L) % g.kv_heads);
+  const int64_t row = x / (2 * L) / g.kv_heads;
+  if (row >= a.n_rows) return;
+  const int32_t seq = a.seq_ids[row], pos = a.positions[row];
+  int32_t bad = 0, page = 0;
+  if (seq < 0 || seq >= a.n_seqs) bad = FAULT_BAD_SEQ;
+  else if (pos < 0 || pos / g.page_tokens >= a.bt_stride) bad = FAULT_BAD_POSITION;
+  else {
+    page = a.bt[(int64_t)seq * a.bt_stride + pos / g.page_tokens];
+    if (page < 0 || page >= g.num_pages) bad = FAULT_BAD_PAGE;
+  }
+  if (bad != 0 && c == 0 && kind == 0 && h == 0) atomicOr(a.fault, bad);
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+  if (bad == 0) {
+    const int slot = pos % g.page_tokens, blk = c / 4;
+    if constexpr (kMx4) {
+      const uint8_t *tile =
+          a.pages + mx4_region_base(g, page, h, kind) + (uint64_t)(slot / 32) * mx4_tile_bytes(D);
+      const int tok = slot % 32;
+      float scale;
+      uint32_t q;
+      if (kind == 0) {
+        const int j = tok % 8 / 4, m = 4 * (tok / 8) + tok % 4, jh = j * (D / 128) + blk / 4;
+        q = *reinterpret_cast<const uint32_t *>(tile + (jh * 4 + blk % 4) * 256 + m * 16 + 4 * (c % 4));
+        const uint32_t s = tile[16 * D + (blk % 4 * 16 + m) * (D / 64) + jh];
+        scale = s == 255 ? __builtin_nanf("") : __builtin_bit_cast(float, s << 23);
+      } else {
+        const int grp = tok / 8, nib = 4 * (tok % 8);
+        q = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // dims 32*blk + 8*(c % 4) + 2*i, +1
+          const v2u w = *reinterpret_cast<const v2u *>(tile + blk / 2 * 1024 + (grp * 16 + 4 * (c % 4) + i) * 16 +
+                                                       8 * (blk % 2));
+          q |= (w[0] >> nib & 15u) << (8 * i) | (w[1] >> nib & 15u) << (8 * i + 4);
+        }
+        const uint32_t s = tile[16 * D + (grp * (D / 32) + blk) * 8 + tok % 8];
+        scale = s >= 0x7c ? __builtin_nanf("") : __builtin_bit_cast(float, (s / 4 - 23 + 127) << 23);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        // 0, 0.5, 1, 1.5, 2, 3, 4, 6: the code as an f32 with one mantissa bit, 0 and 0.5 apart
+        const uint32_t n = q >> (4 * i) & 15u, u = n & 7u;
+        const float m = u < 2 ? 0.5f * (float)u : __builtin_bit_cast(float, (u / 2 + 126u) << 23 | (u & 1u) << 22);
+        v[i] = (n & 8u ? -m : m) * scale;
+      }
+    } else {
+      const uint8_t *region = a.pages + region_base(g, page, h, kind);
+      const float scale = f16_bits_to_f32(*reinterpret_cast<const uint16_t *>(region + scale_offset(g, slot, blk)));
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        v[i] = scale * (float)(int8_t)(region[code_offset(g, kind, slot, 8 * c + i)] ^ code_bias(kind));
+    }
+  }
+  void *out = kind == 0 ? p.k_out : p.v_out;
+  if (out == nullptr) return;
+  const int64_t at = (row * g.kv_heads + h) * D + 8 * c;
+  store4(out, at, p.out_bf16 != 0, v, 0);
+  store4(out, at + 4, p.out_bf16 != 0, v, 4);
+#endif  // __HIP_DEVICE_COMPILE__
+}
+
+// Heads of a query wave: a row's heads over so many waves that the launch has
+// about 4096 (16 a CU), each wave's cosines serving all of its heads.
+int32_t head_chunk(int64_t rows, int32_t heads, int32_t per) {
+  const int64_t want = std::max<int64_t>(1, (int64_t)heads * rows / 4096);
+  return (int32_t)std::min<int64_t>((want + per - 1) / per * per, (heads + per - 1) / per * per);
+}
+
+template <int D, bool kMx4, int ROWS>
+void launch_append_rope_r(const AppendRopeLaunch &p, hipStream_t s) {
+  const int64_t row_blocks = ((int64_t)p.a.n_rows + ROWS - 1) / ROWS;
+  // every head of the rows in one workgroup (their cosines are the same) where that leaves 2 a CU
+  const int32_t H = p.a.g.kv_heads;
+  int32_t heads = H;
+  while (heads > 1 && row_blocks * ((H + heads - 1) / heads) < 2 * kComputeUnits) heads = (heads + 1) / 2;
+  const int32_t groups = (H + heads - 1) / heads;
+  const uint32_t blocks = (uint32_t)(row_blocks * groups);
+  uint32_t q_blocks = 0;
+  int32_t chunk = 1;
+  if (p.q.src != nullptr && p.q.heads > 0) {
+    chunk = head_chunk(p.a.n_rows, p.q.heads, 512 / D);
+    q_blocks = (uint32_t)(((int64_t)p.a.n_rows * ((p.q.heads + chunk - 1) / chunk) + 3) / 4);
+  }
+  if (p.a.src_bf16)
+    hipLaunchKernelGGL((append_rope_kernel<D, kMx4, ROWS, true>), dim3(blocks + q_blocks), dim3(256), 0, s, p, groups,
+                       heads, blocks, chunk);
+  else
+    hipLaunchKernelGGL((append_rope_kernel<D, kMx4, ROWS, false>), dim3(blocks + q_blocks), dim3(256), 0, s, p, groups,
+                       heads, blocks, chunk);
+}
+template <int D, bool kMx4>
+void launch_append_rope_d(const AppendRopeLaunch &p, hipStream_t s) {
+  if ((int64_t)p.a.n_rows * p.a.g.kv_heads >= (int64_t)32 * 8 * kComputeUnits) launch_append_rope_r<D, kMx4, 32>(p, s);
+  else launch_append_rope_r<D, kMx4, 8>(p, s);
+}
+
+}  // namespace
+
+hipError_t launch_rope_rows(const RopeLaunch &r, const HeadRows &q, const HeadRows &k, int32_t head_dim,
+                            hipStream_t s) {
+  if (r.n_rows <= 0 || q.heads + k.heads <= 0) return hipSuccess;
+  const int32_t chunk = head_chunk(r.n_rows, q.heads + k.heads, 512 / head_dim);
+  const int64_t waves = (int64_t)r.n_rows * ((q.heads + chunk - 1) / chunk + (k.heads + chunk - 1) / chunk);
+  const dim3 grid((unsigned)((waves + 3) / 4));
+  if (head_dim == 256) hipLaunchKernelGGL(rope_rows_kernel<256>, grid, dim3(256), 0, s, r, q, k, chunk);
+  else hipLaunchKernelGGL(rope_rows_kernel<128>, grid, dim3(256), 0, s, r, q, k, chunk);
+  return hipGetLastError();
+}
+
+hipError_t launch_append_rope(const AppendRopeLaunch &p, hipStream_t s) {
+  if (p.a.n_rows <= 0) return hipSuccess;
+  if (p.a.g.head_dim == 256) {
+    if (p.mx4) launch_append_rope_d<256, true>(p, s);
+    else launch_append_rope_d<256, false>(p, s);
+  } else {
+    if (p.mx4) launch_append_rope_d<128, true>(p, s);
+    else launch_append_rope_d<128, false>(p, s);
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_read_rows(const ReadRowsLaunch &p, hipStream_t s) {
+  if (p.a.n_rows <= 0) return hipSuccess;
+  const int64_t threads = (int64_t)p.a.n_rows * p.a.g.kv_heads * 2 * (p.a.g.head_dim / 8);
+  const dim3 grid((unsigned)((threads + 255) / 256));
+  if (p.a.g.head_dim == 256) {
+    if (p.mx4) hipLaunchKernelGGL((read_rows_kernel<256, true>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((read_rows_kernel<256, false>), grid, dim3(256), 0, s, p);
+  } else {
+    if (p.mx4) hipLaunchKernelGGL((read_rows_kernel<128, true>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((read_rows_kernel<128, false>), grid, dim3(256), 0, s, p);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace rkv

@@ -775,6 +775,22 @@ rkv_status check_tables(const void *pages, const int32_t *bt, int32_t bt_stride,
   return RKV_OK;
 }
 
+rkv::AppendLaunch make_append(rkv_ctx *ctx, const rkv_kv_geometry *g, void *pages, const int32_t *block_tables,
+                              int32_t bt_stride, int32_t n_seqs, int32_t n_rows, const int32_t *seq_ids,
+                              const int32_t *positions) {
+  rkv::AppendLaunch a{};
+  a.g = to_geo(g);
+  a.pages = static_cast<uint8_t *>(pages);
+  a.bt = block_tables;
+  a.bt_stride = bt_stride;
+  a.n_seqs = n_seqs;
+  a.n_rows = n_rows;
+  a.seq_ids = seq_ids;
+  a.positions = positions;
+  a.fault = ctx->d_fault;
+  return a;
+}
+
 // Split-K plan of a prefill launch: segment length in tokens (0: no split)
 // and the partial rows it writes, rows * q_heads * nseg summed over the
 // entries with more than one segment.  An entry's segment count follows its
@@ -1139,21 +1155,177 @@ rkv_status rkv_append_q8(rkv_ctx *ctx, const rkv_kv_geometry *g, void *pages,
   if (args->n_rows == 0) return RKV_OK;
   if (!args->seq_ids || !args->positions || !args->k_src || !args->v_src)
     return fail(RKV_ERR_INVALID_ARG, op, "NULL seq_ids/positions/k_src/v_src");
-  rkv::AppendLaunch a{};
-  a.g = to_geo(g);
-  a.pages = static_cast<uint8_t *>(pages);
-  a.bt = block_tables;
-  a.bt_stride = bt_stride;
-  a.n_seqs = n_seqs;
-  a.n_rows = args->n_rows;
-  a.seq_ids = args->seq_ids;
-  a.positions = args->positions;
+  rkv::AppendLaunch a = make_append(ctx, g, pages, block_tables, bt_stride, n_seqs, args->n_rows, args->seq_ids,
+                                    args->positions);
   a.k_src = args->k_src;
   a.v_src = args->v_src;
   a.src_bf16 = args->src_dtype == RKV_BF16;
   a.rule = args->rule;
-  a.fault = ctx->d_fault;
   hipError_t e = rkv::launch_append(a, as_stream(stream));
+  return e == hipSuccess ? RKV_OK : hip_fail(op, e);
+}
+
+}  // extern "C"
+
+namespace {
+// Rows of `heads` heads: a pointer and a stride that 16-byte accesses fit.
+rkv_status check_head_rows(const void *p, int64_t stride, int32_t heads, int32_t head_dim, bool bf16,
+                           const char *what, const char *op) {
+  if (!p) return fail(RKV_ERR_INVALID_ARG, op, "%s is NULL", what);
+  const int64_t size = bf16 ? 2 : 4;
+  if (reinterpret_cast<uintptr_t>(p) % 16 != 0 || stride * size % 16 != 0)
+    return fail(RKV_ERR_INVALID_ARG, op, "%s: pointer and row stride must be multiples of 16 bytes", what);
+  if (stride != 0 && stride < (int64_t)heads * head_dim)
+    return fail(RKV_ERR_INVALID_ARG, op, "%s: stride %lld below a row's %lld values", what, (long long)stride,
+                (long long)heads * head_dim);
+  return RKV_OK;
+}
+
+bool dtype_ok(int32_t t) { return t == RKV_F32 || t == RKV_BF16; }
+
+rkv_status check_rope(const rkv_rope_args *r, int32_t head_dim, bool own_positions, const char *op) {
+  if (r->rot_dim < 0 || r->rot_dim > head_dim || r->rot_dim % 8 != 0)
+    return fail(RKV_ERR_INVALID_ARG, op, "rot_dim=%d (a multiple of 8, 0..%d)", r->rot_dim, head_dim);
+  if (r->adjacent != 0 && r->adjacent != 1) return fail(RKV_ERR_INVALID_ARG, op, "adjacent=%d", r->adjacent);
+  if (r->n_axes < 1 || r->n_axes > 4) return fail(RKV_ERR_INVALID_ARG, op, "n_axes=%d (1..4)", r->n_axes);
+  if (r->rot_dim > 0 && !r->freqs) return fail(RKV_ERR_INVALID_ARG, op, "freqs is NULL");
+  if (r->rot_dim > 0 && !r->positions && !(own_positions && r->n_axes == 1))
+    return fail(RKV_ERR_INVALID_ARG, op, "rope positions is NULL");
+  if (r->n_axes > 1 && r->rot_dim > 0 && !r->pair_axis)
+    return fail(RKV_ERR_INVALID_ARG, op, "pair_axis is NULL with %d axes", r->n_axes);
+  if ((r->q_norm || r->k_norm) && !dtype_ok(r->norm_dtype))
+    return fail(RKV_ERR_UNSUPPORTED, op, "norm_dtype=%d", r->norm_dtype);
+  if (!(r->eps >= 0.0f) || !std::isfinite(r->eps)) return fail(RKV_ERR_INVALID_ARG, op, "eps must be finite and >= 0");
+  return RKV_OK;
+}
+
+rkv::RopeLaunch make_rope(const rkv_rope_args *r, int32_t n_rows, int32_t *fault) {
+  rkv::RopeLaunch l{};
+  l.n_rows = n_rows;
+  l.fault = fault;
+  l.n_axes = 1;
+  if (!r) return l;
+  l.on = 1;
+  l.rot_dim = r->rot_dim;
+  l.adjacent = r->adjacent;
+  l.n_axes = r->n_axes;
+  l.freqs = r->freqs;
+  l.pair_axis = r->pair_axis;
+  l.positions = r->positions;
+  l.q_norm = r->q_norm;
+  l.k_norm = r->k_norm;
+  l.norm_bf16 = r->norm_dtype == RKV_BF16;
+  l.eps = r->eps;
+  return l;
+}
+
+rkv_status check_format(const rkv_kv_geometry *g, int32_t format, const char *op) {
+  if (format == RKV_CACHE_Q8) return check_geometry(g, op);
+  if (format == RKV_CACHE_MX4) return check_mx4_geometry(g, op);
+  return fail(RKV_ERR_UNSUPPORTED, op, "format=%d", format);
+}
+}  // namespace
+
+extern "C" {
+
+rkv_status rkv_rope_rows(rkv_ctx *ctx, const rkv_rope_args *rope, const rkv_rope_rows_args *a, void *stream) {
+  const char *op = "rkv_rope_rows";
+  if (!rope || !a) return fail(RKV_ERR_INVALID_ARG, op, "NULL argument");
+  if (a->head_dim != 128 && a->head_dim != 256)
+    return fail(RKV_ERR_UNSUPPORTED, op, "head_dim=%d (built: 128, 256)", a->head_dim);
+  if (a->n_rows < 0 || a->q_heads < 0 || a->kv_heads < 0)
+    return fail(RKV_ERR_INVALID_ARG, op, "n_rows=%d q_heads=%d kv_heads=%d", a->n_rows, a->q_heads, a->kv_heads);
+  if (!dtype_ok(a->src_dtype) || !dtype_ok(a->out_dtype))
+    return fail(RKV_ERR_UNSUPPORTED, op, "src_dtype=%d out_dtype=%d", a->src_dtype, a->out_dtype);
+  if (rkv_status s = check_rope(rope, a->head_dim, false, op)) return s;
+  const bool in16 = a->src_dtype == RKV_BF16, out16 = a->out_dtype == RKV_BF16;
+  const int32_t D = a->head_dim;
+  if (a->n_rows > 0 && a->q_heads > 0) {
+    if (rkv_status s = check_head_rows(a->q_src, a->q_stride, a->q_heads, D, in16, "q_src", op)) return s;
+    if (rkv_status s = check_head_rows(a->q_out, a->q_out_stride, a->q_heads, D, out16, "q_out", op)) return s;
+  }
+  if (a->n_rows > 0 && a->kv_heads > 0) {
+    if (rkv_status s = check_head_rows(a->k_src, a->k_stride, a->kv_heads, D, in16, "k_src", op)) return s;
+    if (rkv_status s = check_head_rows(a->k_out, a->k_out_stride, a->kv_heads, D, out16, "k_out", op)) return s;
+  }
+  if (rkv_status s = use_device(ctx, op)) return s;
+  const rkv::RopeLaunch r = make_rope(rope, a->n_rows, ctx->d_fault);
+  auto stride = [&](int64_t st, int32_t heads) { return st != 0 ? st : (int64_t)heads * D; };
+  const rkv::HeadRows q{a->q_src, a->q_out, stride(a->q_stride, a->q_heads), stride(a->q_out_stride, a->q_heads),
+                        a->q_heads, in16, out16};
+  const rkv::HeadRows k{a->k_src, a->k_out, stride(a->k_stride, a->kv_heads), stride(a->k_out_stride, a->kv_heads),
+                        a->kv_heads, in16, out16};
+  hipError_t e = rkv::launch_rope_rows(r, q, k, D, as_stream(stream));
+  return e == hipSuccess ? RKV_OK : hip_fail(op, e);
+}
+
+rkv_status rkv_append_rope(rkv_ctx *ctx, const rkv_kv_geometry *g, void *pages, const int32_t *block_tables,
+                           int32_t bt_stride, int32_t n_seqs, const rkv_append_rope_args *a, void *stream) {
+  const char *op = "rkv_append_rope";
+  if (!a) return fail(RKV_ERR_INVALID_ARG, op, "args is NULL");
+  if (rkv_status s = check_format(g, a->format, op)) return s;
+  if (rkv_status s = check_tables(pages, block_tables, bt_stride, n_seqs, op)) return s;
+  if (a->n_rows < 0) return fail(RKV_ERR_INVALID_ARG, op, "n_rows=%d", a->n_rows);
+  if (!dtype_ok(a->src_dtype)) return fail(RKV_ERR_UNSUPPORTED, op, "src_dtype=%d", a->src_dtype);
+  if (a->rule != 0 && !(a->format == RKV_CACHE_Q8 && a->rule == RKV_Q8_HARSERVE))
+    return fail(RKV_ERR_INVALID_ARG, op, "rule=%d", a->rule);
+  const int32_t D = g->head_dim;
+  if (a->rope)
+    if (rkv_status s = check_rope(a->rope, D, true, op)) return s;
+  const bool in16 = a->src_dtype == RKV_BF16;
+  const bool with_q = a->q_src != nullptr;
+  if (with_q && (a->q_heads < 1 || !dtype_ok(a->q_out_dtype)))
+    return fail(RKV_ERR_INVALID_ARG, op, "q_heads=%d q_out_dtype=%d", a->q_heads, a->q_out_dtype);
+  if (a->n_rows > 0) {
+    if (!a->seq_ids || !a->positions) return fail(RKV_ERR_INVALID_ARG, op, "NULL seq_ids/positions");
+    if (rkv_status s = check_head_rows(a->k_src, a->k_stride, g->kv_heads, D, in16, "k_src", op)) return s;
+    if (rkv_status s = check_head_rows(a->v_src, a->v_stride, g->kv_heads, D, in16, "v_src", op)) return s;
+    if (with_q) {
+      if (rkv_status s = check_head_rows(a->q_src, a->q_stride, a->q_heads, D, in16, "q_src", op)) return s;
+      if (rkv_status s = check_head_rows(a->q_out, 0, a->q_heads, D, a->q_out_dtype == RKV_BF16, "q_out", op)) return s;
+    }
+  }
+  if (rkv_status s = use_device(ctx, op)) return s;
+  if (a->n_rows == 0) return RKV_OK;
+  rkv::AppendRopeLaunch l{};
+  l.a = make_append(ctx, g, pages, block_tables, bt_stride, n_seqs, a->n_rows, a->seq_ids, a->positions);
+  l.a.k_src = a->k_src;
+  l.a.v_src = a->v_src;
+  l.a.src_bf16 = in16;
+  l.a.rule = a->rule;
+  auto stride = [&](int64_t st, int32_t heads) { return st != 0 ? st : (int64_t)heads * D; };
+  l.k_stride = stride(a->k_stride, g->kv_heads);
+  l.v_stride = stride(a->v_stride, g->kv_heads);
+  l.mx4 = a->format == RKV_CACHE_MX4;
+  l.r = make_rope(a->rope, a->n_rows, ctx->d_fault);
+  if (with_q)
+    l.q = rkv::HeadRows{a->q_src, a->q_out, stride(a->q_stride, a->q_heads), (int64_t)a->q_heads * D, a->q_heads,
+                        in16, a->q_out_dtype == RKV_BF16};
+  hipError_t e = rkv::launch_append_rope(l, as_stream(stream));
+  return e == hipSuccess ? RKV_OK : hip_fail(op, e);
+}
+
+rkv_status rkv_read_rows(rkv_ctx *ctx, const rkv_kv_geometry *g, int32_t format, const void *pages,
+                         const int32_t *block_tables, int32_t bt_stride, int32_t n_seqs, int32_t n_rows,
+                         const int32_t *seq_ids, const int32_t *positions, void *k_out, void *v_out,
+                         int32_t out_dtype, void *stream) {
+  const char *op = "rkv_read_rows";
+  if (rkv_status s = check_format(g, format, op)) return s;
+  if (rkv_status s = check_tables(pages, block_tables, bt_stride, n_seqs, op)) return s;
+  if (n_rows < 0) return fail(RKV_ERR_INVALID_ARG, op, "n_rows=%d", n_rows);
+  if (!dtype_ok(out_dtype)) return fail(RKV_ERR_UNSUPPORTED, op, "out_dtype=%d", out_dtype);
+  if (n_rows > 0 && (!seq_ids || !positions)) return fail(RKV_ERR_INVALID_ARG, op, "NULL seq_ids/positions");
+  if (reinterpret_cast<uintptr_t>(k_out) % 16 != 0 || reinterpret_cast<uintptr_t>(v_out) % 16 != 0)
+    return fail(RKV_ERR_INVALID_ARG, op, "k_out and v_out must be multiples of 16 bytes");
+  if (rkv_status s = use_device(ctx, op)) return s;
+  if (n_rows == 0 || (!k_out && !v_out)) return RKV_OK;
+  rkv::ReadRowsLaunch l{};
+  l.a = make_append(ctx, g, const_cast<void *>(pages), block_tables, bt_stride, n_seqs, n_rows, seq_ids, positions);
+  l.mx4 = format == RKV_CACHE_MX4;
+  l.k_out = k_out;
+  l.v_out = v_out;
+  l.out_bf16 = out_dtype == RKV_BF16;
+  hipError_t e = rkv::launch_read_rows(l, as_stream(stream));
   return e == hipSuccess ? RKV_OK : hip_fail(op, e);
 }
 

@@ -1,0 +1,127 @@
+"""CPU checks of the rotation's entry points: every refusal comes before any
+device work, so they run here with no context and pointers never followed."""
+import ctypes as C
+
+import pytest
+
+import mx4_ref  # noqa: F401  (the oracle imports on its own)
+
+
+def _rope(rkv, **over):
+    r = rkv.RopeArgs(128, 0, 64, 1, None, 64, None, None, rkv.F32, 1e-6)
+    for k, v in over.items():
+        setattr(r, k, v)
+    return r
+
+
+def _rows(rkv, rope=None, **over):
+    a = rkv.RopeRowsArgs(3, 128, 4, 2, 64, 64, 0, 0, rkv.BF16, 64, 64, 0, 0, rkv.BF16)
+    for k, v in over.items():
+        setattr(a, k, v)
+    rope = rope or _rope(rkv)
+    return rkv.lib().rkv_rope_rows(None, C.byref(rope), C.byref(a), None), rkv.lib().rkv_last_error().decode()
+
+
+@pytest.mark.parametrize("rope,rows,status,text", [
+    ({}, {}, -1, "ctx is NULL"),
+    ({"rot_dim": 12}, {}, -1, "rot_dim=12"),
+    ({"rot_dim": 136}, {}, -1, "rot_dim=136"),
+    ({"adjacent": 2}, {}, -1, "adjacent=2"),
+    ({"n_axes": 5}, {}, -1, "n_axes=5"),
+    ({"n_axes": 3}, {}, -1, "pair_axis"),
+    ({"freqs": None}, {}, -1, "freqs"),
+    ({"positions": None}, {}, -1, "positions"),
+    ({"q_norm": 64, "norm_dtype": 7}, {}, -4, "norm_dtype"),
+    ({"eps": -1.0}, {}, -1, "eps"),
+    ({"eps": float("nan")}, {}, -1, "eps"),
+    ({}, {"head_dim": 64}, -4, "head_dim=64"),
+    ({}, {"n_rows": -1}, -1, "n_rows=-1"),
+    ({}, {"src_dtype": 5}, -4, "src_dtype=5"),
+    ({}, {"q_src": None}, -1, "q_src is NULL"),
+    ({}, {"q_src": 66}, -1, "16 bytes"),
+    ({}, {"k_stride": 260}, -1, "16 bytes"),
+    ({}, {"k_stride": 248}, -1, "stride 248"),
+    ({}, {"q_out": 72}, -1, "q_out"),
+])
+def test_rope_rows_refusals(rkv, rope, rows, status, text):
+    st, msg = _rows(rkv, _rope(rkv, **rope), **rows)
+    assert st == status and text in msg and msg.startswith("rkv_rope_rows"), msg
+
+
+def test_no_rotation_needs_no_positions(rkv):
+    st, msg = _rows(rkv, _rope(rkv, rot_dim=0, freqs=None, positions=None, q_norm=64))
+    assert "ctx is NULL" in msg
+
+
+def _append(rkv, g, **over):
+    rope = _rope(rkv)
+    a = rkv.AppendRopeArgs(5, 64, 64, 64, 64, 0, 0, rkv.BF16, rkv.CACHE_MX4, 0, C.pointer(rope), 64, 0, 8, 64,
+                           rkv.BF16)
+    for k, v in over.items():
+        setattr(a, k, v)
+    st = rkv.lib().rkv_append_rope(None, C.byref(g), 64, 64, 4, 2, C.byref(a), None)
+    return st, rkv.lib().rkv_last_error().decode()
+
+
+@pytest.mark.parametrize("over,status,text", [
+    ({}, -1, "ctx is NULL"),
+    ({"format": 2}, -4, "format=2"),
+    ({"rule": 1}, -1, "rule=1"),
+    ({"n_rows": -2}, -1, "n_rows=-2"),
+    ({"seq_ids": None}, -1, "seq_ids"),
+    ({"v_src": None}, -1, "v_src"),
+    ({"k_stride": 128}, -1, "stride 128"),
+    ({"q_heads": 0}, -1, "q_heads=0"),
+    ({"q_out_dtype": 9}, -1, "q_out_dtype=9"),
+    ({"q_out": None}, -1, "q_out is NULL"),
+    ({"src_dtype": 3}, -4, "src_dtype=3"),
+])
+def test_append_refusals(rkv, over, status, text):
+    st, msg = _append(rkv, rkv.geometry(2, 128, 32, 10), **over)
+    assert st == status and text in msg and msg.startswith("rkv_append_rope"), msg
+
+
+def test_append_formats_and_pages(rkv):
+    g16 = rkv.geometry(2, 128, 16, 10)
+    st, msg = _append(rkv, g16)
+    assert st == -4 and "page_tokens=16" in msg
+    st, msg = _append(rkv, g16, format=rkv.CACHE_Q8, rule=rkv.Q8_HARSERVE)
+    assert "ctx is NULL" in msg
+
+
+def test_read_rows_refusals(rkv):
+    g = rkv.geometry(2, 128, 32, 10)
+
+    def read(g=g, fmt=rkv.CACHE_MX4, n=3, seqs=64, k=64, dtype=rkv.F32):
+        st = rkv.lib().rkv_read_rows(None, C.byref(g), fmt, 64, 64, 4, 2, n, seqs, 64, k, 64, dtype, None)
+        return st, rkv.lib().rkv_last_error().decode()
+    assert "ctx is NULL" in read()[1]
+    assert read(fmt=5)[0] == -4 and read(n=-1)[0] == -1 and read(seqs=None)[0] == -1
+    assert read(k=72)[0] == -1 and read(dtype=2)[0] == -4
+    assert read(g=rkv.geometry(2, 128, 16, 10))[0] == -4
+
+
+def test_binding_refuses_what_it_would_misread(rkv):
+    import torch
+    f = torch.ones(64)
+    pos = torch.zeros(3, dtype=torch.int32)
+    rope = rkv.rope_args(128, f, pos)
+    q = torch.zeros(3, 4, 128)
+    with pytest.raises(TypeError):
+        rkv.rope_args(128, f.double(), pos)
+    with pytest.raises(TypeError):
+        rkv.rope_args(128, f, pos.long())
+    with pytest.raises(ValueError):
+        rkv.rope_args(64, f, pos)
+
+    class Ctx:
+        h = None
+    for bad in (q.half(), ):
+        with pytest.raises((TypeError, ValueError)):
+            rkv.rope_rows(Ctx, rope, bad, None, bad, None)
+    with pytest.raises(ValueError):  # heads apart
+        rkv.rope_rows(Ctx, rope, torch.zeros(3, 8, 128)[:, ::2], None, q, None)
+    with pytest.raises(ValueError):  # other rows than positions
+        rkv.rope_rows(Ctx, rope, torch.zeros(4, 4, 128), None, torch.zeros(4, 4, 128), None)
+    with pytest.raises(ValueError):
+        rkv.append_rope_args(rkv.CACHE_MX4, pos, pos, q, q[:, :2])

@@ -367,6 +367,16 @@ rkv_status rkv_decode_mx4(rkv_ctx *ctx, const rkv_kv_geometry *g, const void *pa
  * partition_tokens 0 it does not fall as batch or max_seq_len grows. */
 size_t rkv_decode_mx4_workspace_bytes(const rkv_kv_geometry *g, const rkv_decode_args *args);
 
+/* rkv_prefill_q8 over 4-bit pages, with a bf16 query (q_dtype RKV_F32 is
+ * RKV_ERR_UNSUPPORTED): the same arguments, split and faults.  f32 rows carry
+ * their softmax weights in 22 bits, bf16 rows in 11.  NaN blocks as in
+ * rkv_decode_mx4. */
+rkv_status rkv_prefill_mx4(rkv_ctx *ctx, const rkv_kv_geometry *g, const void *pages,
+                           const int32_t *block_tables, int32_t bt_stride, int32_t n_seqs,
+                           const rkv_prefill_args *args, void *stream);
+/* Workspace bytes of its split (0 when there is none). */
+size_t rkv_prefill_mx4_workspace_bytes(const rkv_kv_geometry *g, const rkv_prefill_args *args);
+
 /* ---- norm and position rotation ---------------------------------------------
  * Query and key rows as a model's projections give them, normed head by head
  * and rotated by their positions, in one pass:

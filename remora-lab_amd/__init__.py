@@ -223,6 +223,9 @@ _SIGS = {
     "rkv_prefill_q8": (C.c_int32, [P, C.POINTER(Geometry), P, P, C.c_int32, C.c_int32,
                                    C.POINTER(PrefillArgs), P]),
     "rkv_pool_prefill": (C.c_int32, [P, C.c_int32, C.POINTER(PrefillArgs), P]),
+    "rkv_prefill_mx4": (C.c_int32, [P, C.POINTER(Geometry), P, P, C.c_int32, C.c_int32,
+                                    C.POINTER(PrefillArgs), P]),
+    "rkv_prefill_mx4_workspace_bytes": (C.c_size_t, [C.POINTER(Geometry), C.POINTER(PrefillArgs)]),
     "rkv_crc32c_host": (C.c_uint32, [P, C.c_size_t]),
     "rkv_crc32c": (C.c_int32, [P, P, C.c_uint64, P, P]),
     "rkv_r4kv_header_encode": (C.c_int32, [C.POINTER(R4kvHeader), P]),
@@ -516,6 +519,17 @@ def prefill_q8(ctx: Ctx, g: Geometry, pages, block_tables, n_seqs: int, a: Prefi
                stream=None) -> None:
     check(lib().rkv_prefill_q8(ctx.h, C.byref(g), _ptr(pages), _ptr(block_tables),
                                block_tables.shape[1], n_seqs, C.byref(a), _stream(stream)))
+
+
+def prefill_mx4_workspace_bytes(g: Geometry, a: PrefillArgs) -> int:
+    return lib().rkv_prefill_mx4_workspace_bytes(C.byref(g), C.byref(a))
+
+
+def prefill_mx4(ctx: Ctx, g: Geometry, pages, block_tables, n_seqs: int, a: PrefillArgs,
+                stream=None) -> None:
+    """rkv_prefill_q8 over 4-bit pages (a bf16 query)."""
+    check(lib().rkv_prefill_mx4(ctx.h, C.byref(g), _ptr(pages), _ptr(block_tables),
+                                block_tables.shape[1], n_seqs, C.byref(a), _stream(stream)))
 
 
 def _host_buf(data):

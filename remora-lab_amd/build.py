@@ -15,8 +15,8 @@ CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "librkv.so")
 OBJDIR = os.path.join(HERE, "_build")
 
-SOURCES = ["rkv_append.hip", "rkv_decode.hip", "rkv_decode_rows32.hip", "rkv_mx4_decode.hip", "rkv_rope.hip",
-           "rkv_prefill.hip",
+SOURCES = ["rkv_append.hip", "rkv_decode.hip", "rkv_decode_rows32.hip", "rkv_mx4_decode.hip", "rkv_mx4_prefill.hip",
+           "rkv_rope.hip", "rkv_prefill.hip",
            "rkv_r4kv.hip", "rkv_stream.hip", "rkv_scratch.hip", "rkv_runtime.cpp", "rkv_serve.cpp"]
 
 # Per-file extra flags.  rkv_decode.hip: MFMA destinations and accumulators
@@ -24,7 +24,8 @@ SOURCES = ["rkv_append.hip", "rkv_decode.hip", "rkv_decode_rows32.hip", "rkv_mx4
 # two-wave 32-row variant (rkv_decode_rows32.hip) is bounded to 256 registers
 # per wave by its launch bounds and allocates no AGPRs either way.
 # rkv_mx4_decode.hip: without it the 17..32-row variant at head_dim 256 spills.
-EXTRA = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for f in ("rkv_decode.hip", "rkv_mx4_decode.hip")}
+EXTRA = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for f in ("rkv_decode.hip", "rkv_mx4_decode.hip",
+                                                            "rkv_mx4_prefill.hip")}
 
 # -packed-fp32-ops off: no v_pk_*_f32 are generated (unreliable on this pool).
 # f32 division and sqrt stay correctly rounded and f32 denormals are kept, so

@@ -209,6 +209,10 @@ struct PrefillLaunch {
   int64_t preoff[kPrefillMaxEntries + 1];
 };
 hipError_t launch_prefill(const PrefillLaunch &pf, hipStream_t s);
+// the merge of its split entries' partials, which launch_prefill ends with
+hipError_t launch_prefill_combine(const PrefillLaunch &pf, hipStream_t s);
+// The same over 4-bit pages with a bf16 query (pf.pre has no part in it).
+hipError_t launch_mx4_prefill(const PrefillLaunch &pf, hipStream_t s);
 // bytes of one widened tile image: K and V f16 (64*D each), the K and V
 // scale runs (2*D each), padded to whole 1 KiB copies
 constexpr int64_t prefill_tile_bytes(int head_dim) { return (132LL * head_dim + 1023) / 1024 * 1024; }

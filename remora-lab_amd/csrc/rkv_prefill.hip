@@ -361,27 +361,9 @@ __global__ __launch_bounds__(64) void prefill_combine_kernel(PrefillCombine c) {
   }
 }
 
-template <int D, int NS>
-hipError_t launch_prefill_t(const PrefillLaunch &pf, hipStream_t s) {
-  const int64_t units = (int64_t)pf.first[pf.n_entries] * pf.d.g.kv_heads;
-  const int64_t round = 8 * (int64_t)std::max(pf.xcd_chunk, 1);
-  dim3 grid((unsigned)((units + round - 1) / round * round));
-  const bool small = pf.d.g.page_tokens < kTile, qf16 = pf.d.q_bf16 != 0;
-  if (pf.pre != nullptr && qf16) {
-    // widen every tile once, then copy the images
-    hipLaunchKernelGGL(widen_tiles_kernel<D>, dim3((unsigned)pf.preoff[pf.n_entries]), dim3(256), 0, s, pf);
-    hipLaunchKernelGGL((prefill_kernel<D, false, NS, true, true>), grid, dim3(64 * kPrefillWaves), 0, s, pf);
-  } else if (small && qf16)
-    hipLaunchKernelGGL((prefill_kernel<D, true, NS, true>), grid, dim3(64 * kPrefillWaves), 0, s, pf);
-  else if (small)
-    hipLaunchKernelGGL((prefill_kernel<D, true, NS, false>), grid, dim3(64 * kPrefillWaves), 0, s, pf);
-  else if (qf16)
-    hipLaunchKernelGGL((prefill_kernel<D, false, NS, true>), grid, dim3(64 * kPrefillWaves), 0, s, pf);
-  else
-    hipLaunchKernelGGL((prefill_kernel<D, false, NS, false>), grid, dim3(64 * kPrefillWaves), 0, s, pf);
-  hipError_t err = hipGetLastError();
-  if (err != hipSuccess) return err;
-  // merge the split entries' partials into their rows
+// Merges the split entries' partials into their rows.
+template <int D>
+hipError_t launch_combine_t(const PrefillLaunch &pf, hipStream_t s) {
   PrefillCombine c{};
   c.q_heads = pf.d.q_heads;
   c.out_bf16 = pf.d.out_bf16;
@@ -404,12 +386,39 @@ hipError_t launch_prefill_t(const PrefillLaunch &pf, hipStream_t s) {
   return hipGetLastError();
 }
 
+template <int D, int NS>
+hipError_t launch_prefill_t(const PrefillLaunch &pf, hipStream_t s) {
+  const int64_t units = (int64_t)pf.first[pf.n_entries] * pf.d.g.kv_heads;
+  const int64_t round = 8 * (int64_t)std::max(pf.xcd_chunk, 1);
+  dim3 grid((unsigned)((units + round - 1) / round * round));
+  const bool small = pf.d.g.page_tokens < kTile, qf16 = pf.d.q_bf16 != 0;
+  if (pf.pre != nullptr && qf16) {
+    // widen every tile once, then copy the images
+    hipLaunchKernelGGL(widen_tiles_kernel<D>, dim3((unsigned)pf.preoff[pf.n_entries]), dim3(256), 0, s, pf);
+    hipLaunchKernelGGL((prefill_kernel<D, false, NS, true, true>), grid, dim3(64 * kPrefillWaves), 0, s, pf);
+  } else if (small && qf16)
+    hipLaunchKernelGGL((prefill_kernel<D, true, NS, true>), grid, dim3(64 * kPrefillWaves), 0, s, pf);
+  else if (small)
+    hipLaunchKernelGGL((prefill_kernel<D, true, NS, false>), grid, dim3(64 * kPrefillWaves), 0, s, pf);
+  else if (qf16)
+    hipLaunchKernelGGL((prefill_kernel<D, false, NS, true>), grid, dim3(64 * kPrefillWaves), 0, s, pf);
+  else
+    hipLaunchKernelGGL((prefill_kernel<D, false, NS, false>), grid, dim3(64 * kPrefillWaves), 0, s, pf);
+  hipError_t err = hipGetLastError();
+  if (err != hipSuccess) return err;
+  return launch_combine_t<D>(pf, s);
+}
+
 }  // namespace
 
 hipError_t launch_prefill(const PrefillLaunch &pf, hipStream_t s) {
   if (pf.n_entries <= 0 || pf.first[pf.n_entries] <= 0) return hipSuccess;
   if (pf.d.g.head_dim == 256) return launch_prefill_t<256, 2>(pf, s);
   return launch_prefill_t<128, 2>(pf, s);
+}
+
+hipError_t launch_prefill_combine(const PrefillLaunch &pf, hipStream_t s) {
+  return pf.d.g.head_dim == 256 ? launch_combine_t<256>(pf, s) : launch_combine_t<128>(pf, s);
 }
 
 }  // namespace rkv

@@ -1080,7 +1080,7 @@ rkv_status make_prefill(rkv_ctx *ctx, const rkv_kv_geometry *g, const void *page
   d.scale_log2 = a->scale * 1.4426950408889634f;
   d.out = a->out;
   d.out_bf16 = a->out_dtype == RKV_BF16;
-  d.fault = ctx->d_fault;
+  d.fault = ctx ? ctx->d_fault : nullptr;
   d.stages = 2;
   return RKV_OK;
 }
@@ -1113,6 +1113,8 @@ rkv_status rkv_prefill_q8(rkv_ctx *ctx, const rkv_kv_geometry *g, const void *pa
 }  // extern "C"
 
 namespace {
+constexpr int32_t kMx4PrefillXcdChunk = rkv::kPrefillXcdChunkHbm;
+
 // Workspace of a prefill launched with this XCD chunk (the split plan's
 // dispatch simulation depends on it), with room for the widened tiles when
 // the launch would widen once (HBM pages and a bf16 query).
@@ -1134,6 +1136,26 @@ size_t prefill_ws_query(const rkv_kv_geometry *g, const rkv_prefill_args *a, int
 }  // namespace
 
 extern "C" {
+
+size_t rkv_prefill_mx4_workspace_bytes(const rkv_kv_geometry *g, const rkv_prefill_args *a) {
+  if (check_mx4_geometry(g, "rkv_prefill_mx4_workspace_bytes") != RKV_OK) return 0;
+  return prefill_ws_query(g, a, kMx4PrefillXcdChunk, false);
+}
+
+rkv_status rkv_prefill_mx4(rkv_ctx *ctx, const rkv_kv_geometry *g, const void *pages,
+                           const int32_t *block_tables, int32_t bt_stride, int32_t n_seqs,
+                           const rkv_prefill_args *a, void *stream) {
+  const char *op = "rkv_prefill_mx4";
+  if (rkv_status s = check_mx4_geometry(g, op)) return s;
+  rkv::PrefillLaunch pf{};
+  if (rkv_status s = make_prefill(ctx, g, pages, block_tables, bt_stride, n_seqs, a, op, kMx4PrefillXcdChunk, false, pf))
+    return s;
+  if (a->q_dtype != RKV_BF16) return fail(RKV_ERR_UNSUPPORTED, op, "q_dtype=%d (built for 4-bit pages: bf16)", a->q_dtype);
+  if (rkv_status s = use_device(ctx, op)) return s;
+  pf.d.fault = ctx->d_fault;
+  hipError_t e = rkv::launch_mx4_prefill(pf, as_stream(stream));
+  return e == hipSuccess ? RKV_OK : hip_fail(op, e);
+}
 
 size_t rkv_prefill_workspace_bytes(const rkv_kv_geometry *g, const rkv_prefill_args *a) {
   return prefill_ws_query(g, a, rkv::kPrefillXcdChunkHbm, true);

@@ -83,3 +83,32 @@ def test_decode_workspace(rkv):
         return rkv.decode_mx4_workspace_bytes(g, a)
     assert need(64, 512) == 0 and need(1, 1) == 0 and need(1, 513) > 0
     assert need(1, 600) <= need(1, 4096) <= need(4, 4096) <= need(64, 32768)
+
+
+def _prefill(rkv, g, **over):
+    one = [(C.c_int32 * 1)(v) for v in (0, 100, 7, 0)]
+    a = rkv.PrefillArgs(1, *[C.cast(x, rkv.I32P) for x in one], 7, 64, rkv.BF16, 8, 0.1, 64, rkv.F32, 0, None, 0)
+    for k, v in over.items():
+        setattr(a, k, v)
+    st = rkv.lib().rkv_prefill_mx4(None, C.byref(g), 64, 64, 8, 2, C.byref(a), None)
+    return st, rkv.lib().rkv_last_error().decode()
+
+
+@pytest.mark.parametrize("over,status,text", [
+    ({}, -1, "ctx is NULL"),
+    ({"q_dtype": 0}, -4, "bf16"),
+    ({"q_heads": 3}, -1, "q_heads=3"),
+    ({"total_rows": 3}, -1, "total_rows=3"),
+    ({"n_seqs": 65}, -1, "n_seqs=65"),
+    ({"segment_tokens": 64}, -1, "workspace"),
+    ({"workspace": 100}, -1, "256-byte"),
+    ({"out": None}, -1, "NULL q/out"),
+])
+def test_prefill_refusals(rkv, over, status, text):
+    st, msg = _prefill(rkv, rkv.geometry(2, 256, 64, 10), **over)
+    assert st == status and text in msg and msg.startswith("rkv_prefill_mx4"), msg
+
+
+def test_prefill_refuses_small_pages(rkv):
+    st, msg = _prefill(rkv, rkv.geometry(2, 256, 16, 10))
+    assert st == -4 and "page_tokens=16" in msg

@@ -529,7 +529,7 @@ def prefill_mx4(ctx: Ctx, g: Geometry, pages, block_tables, n_seqs: int, a: Pref
                 stream=None) -> None:
     """rkv_prefill_q8 over 4-bit pages (a bf16 query)."""
     check(lib().rkv_prefill_mx4(ctx.h, C.byref(g), _ptr(pages), _ptr(block_tables),
-                                block_tables.shape[1], n_seqs, C.byref(a), _stream(stream)))
+                                block_tables.shape[1], n_seqs, C.byref(a), _raw_stream(ctx, stream)))
 
 
 def _host_buf(data):
@@ -640,26 +640,55 @@ def decode_q8_noalloc(ctx: Ctx, g: Geometry, pages, block_tables, seq_lens, a: D
                                       C.byref(a), _stream(stream)))
 
 
-def _dtype(t) -> int:
-    """The RKV_* type of a tensor; others are refused here, their bytes would be misread."""
-    import torch
-    if t.dtype not in (torch.float32, torch.bfloat16):
-        raise TypeError(f"float32 or bfloat16 wanted, got {t.dtype}")
-    return BF16 if t.dtype == torch.bfloat16 else F32
+_torch = None
+_types: dict = {}  # torch dtype -> RKV_* type
 
 
-def _i32(t, what: str):
+def _load_torch():
+    global _torch
     import torch
-    if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
+    _types.update({torch.float32: F32, torch.bfloat16: BF16})
+    _torch = torch
+    return torch
+
+
+def _type(dtype) -> int:
+    if _torch is None:
+        _load_torch()
+    try:
+        return _types[dtype]
+    except KeyError:
+        raise TypeError(f"float32 or bfloat16 wanted, got {dtype}") from None
+
+
+def _raw_stream(ctx: Ctx, s):
+    """Handle of a stream, None: the current one of the context's device."""
+    if s is None:
+        return (_torch or _load_torch())._C._cuda_getCurrentRawStream(ctx.device)
+    return s if isinstance(s, int) else s.cuda_stream
+
+
+def _i32(t, what: str) -> int | None:
+    """Address of a contiguous int32 tensor (or None)."""
+    if t is None:
+        return None
+    if t.dtype is not (_torch or _load_torch()).int32 or not t.is_contiguous():
         raise TypeError(f"{what}: a contiguous int32 tensor wanted")
-    return t
+    return t.data_ptr()
 
 
-def _head_rows(t, what: str) -> int:
-    """Row stride of [rows][heads][head_dim] values whose heads lie one after the other."""
-    if t.dim() != 3 or t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
-        raise ValueError(f"{what}: [rows][heads][head_dim] with dense heads wanted")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+def _heads(t, n: int, D: int, dtype, what: str, device: int) -> tuple[int, int, int]:
+    """(address, heads, row stride) of t [n][heads][D], whose heads lie one after
+    the other.  Anything else is refused: its bytes would be misread."""
+    r, h, d = t.shape
+    s0, s1, s2 = t.stride()
+    if r != n or d != D or t.dtype != dtype:
+        raise ValueError(f"{what}: [{n}][heads][{D}] of {dtype} wanted, got {tuple(t.shape)} of {t.dtype}")
+    if s2 != 1 or (h > 1 and s1 != D):
+        raise ValueError(f"{what}: dense heads wanted, got strides {t.stride()}")
+    if t.get_device() != device:
+        raise ValueError(f"{what}: a tensor of device {device} wanted")
+    return t.data_ptr(), h, s0 if n > 1 else h * D
 
 
 def rope_args(rot_dim: int, freqs, positions=None, pair_axis=None, adjacent: bool = False, q_norm=None,
@@ -676,94 +705,96 @@ def rope_args(rot_dim: int, freqs, positions=None, pair_axis=None, adjacent: boo
     norms = [w for w in (q_norm, k_norm) if w is not None]
     if any(not w.is_contiguous() or w.dtype != norms[0].dtype for w in norms):
         raise TypeError("q_norm and k_norm: contiguous, of one type")
-    a = RopeArgs(rot_dim, int(adjacent), _ptr(freqs), n_axes, _ptr(_i32(pair_axis, "pair_axis")),
-                 _ptr(_i32(positions, "positions")), _ptr(q_norm), _ptr(k_norm),
-                 _dtype(norms[0]) if norms else F32, eps)
+    a = RopeArgs(rot_dim, int(adjacent), _ptr(freqs), n_axes, _i32(pair_axis, "pair_axis"),
+                 _i32(positions, "positions"), _ptr(q_norm), _ptr(k_norm),
+                 _type(norms[0].dtype) if norms else F32, eps)
     a._refs = (freqs, positions, pair_axis, q_norm, k_norm)
     a._rows = None if positions is None else positions.shape[-1]
+    a._dims = [None if w is None else w.numel() for w in (q_norm, k_norm)]
     return a
 
 
-def _rope_fits(rope, n_rows: int, *heads) -> None:
-    if rope is None:
-        return
-    if rope._rows is not None and rope._rows != n_rows:
-        raise ValueError(f"{rope._rows} rope positions for {n_rows} rows")
-    for w, t in heads:
-        if w is not None and t is not None and w.numel() != t.shape[2]:
-            raise ValueError("a norm weight has head_dim values")
+def _rope_fits(rope: RopeArgs, n: int, D: int) -> None:
+    if rope._rows is not None and rope._rows != n:
+        raise ValueError(f"{rope._rows} rope positions for {n} rows")
+    if rope._dims[0] not in (None, D) or rope._dims[1] not in (None, D):
+        raise ValueError("a norm weight has head_dim values")
 
 
 def rope_rows(ctx: Ctx, rope: RopeArgs, q, k, q_out, k_out, stream=None) -> None:
     """Norm and rotation of q and k [rows][heads][head_dim] (views with any row
     stride; either may be None) into q_out and k_out of the same shapes."""
-    one = q if q is not None else k
-    n, D = one.shape[0], one.shape[2]
-    for t, o in ((q, q_out), (k, k_out)):
-        if t is not None and (t.shape != o.shape or t.shape[0] != n or t.shape[2] != D or t.dtype != one.dtype):
-            raise ValueError("q, k and their outputs: one number of rows, head_dim and type, shapes alike")
-    outs = [o for t, o in ((q, q_out), (k, k_out)) if t is not None]
-    if any(o.dtype != outs[0].dtype for o in outs):
-        raise ValueError("q_out and k_out have one type")
-    _rope_fits(rope, n, (rope._refs[3], q), (rope._refs[4], k))
-    a = RopeRowsArgs(n, D, q.shape[1] if q is not None else 0, k.shape[1] if k is not None else 0,
-                     _ptr(q), _ptr(k), _head_rows(q, "q") if q is not None else 0,
-                     _head_rows(k, "k") if k is not None else 0, _dtype(one),
-                     _ptr(q_out) if q is not None else None, _ptr(k_out) if k is not None else None,
-                     _head_rows(q_out, "q_out") if q is not None else 0,
-                     _head_rows(k_out, "k_out") if k is not None else 0, _dtype(outs[0]))
-    check(lib().rkv_rope_rows(ctx.h, C.byref(rope), C.byref(a), _stream(stream)))
-
-
-def append_rope_args(fmt: int, seq_ids, positions, k_src, v_src, rope: RopeArgs | None = None, q=None,
-                     q_out=None, rule: int = Q8_CANONICAL) -> AppendRopeArgs:
-    """Rows [n][kv_heads][head_dim] (views with any row stride) of one append;
-    q [n][q_heads][head_dim] goes normed and rotated to q_out (contiguous)."""
-    n = seq_ids.numel()
-    for t in (k_src, v_src, q):
-        if t is not None and (t.shape[0] != n or t.shape[2] != k_src.shape[2] or t.dtype != k_src.dtype):
-            raise ValueError("k, v and q: one number of rows, head_dim and type")
-    if v_src.shape != k_src.shape or positions.numel() != n:
-        raise ValueError("v and positions go with k")
-    if q is not None and (q_out.shape != q.shape or not q_out.is_contiguous()):
-        raise ValueError("q_out: contiguous, shaped like q")
-    if rope is not None:
-        _rope_fits(rope, n, (rope._refs[3], q), (rope._refs[4], k_src))
-    a = AppendRopeArgs(n, _ptr(_i32(seq_ids, "seq_ids")), _ptr(_i32(positions, "positions")), _ptr(k_src), _ptr(v_src),
-                       _head_rows(k_src, "k"), _head_rows(v_src, "v"), _dtype(k_src), fmt, rule,
-                       C.pointer(rope) if rope is not None else None, _ptr(q),
-                       _head_rows(q, "q") if q is not None else 0, q.shape[1] if q is not None else 0,
-                       _ptr(q_out) if q is not None else None, _dtype(q_out) if q is not None else F32)
-    a._refs = (seq_ids, positions, k_src, v_src, rope, q, q_out)
-    a._heads = k_src.shape[1:]
-    return a
+    one, out = (q, q_out) if q is not None else (k, k_out)
+    n, _, D = one.shape
+    dtype, otype, dev = one.dtype, out.dtype, ctx.device
+    _rope_fits(rope, n, D)
+    qp, qh, qs, qo, qos = None, 0, 0, None, 0
+    kp, kh, ks, ko, kos = None, 0, 0, None, 0
+    if q is not None:
+        qp, qh, qs = _heads(q, n, D, dtype, "q", dev)
+        qo, h, qos = _heads(q_out, n, D, otype, "q_out", dev)
+        if h != qh:
+            raise ValueError("q_out has q's heads")
+    if k is not None:
+        kp, kh, ks = _heads(k, n, D, dtype, "k", dev)
+        ko, h, kos = _heads(k_out, n, D, otype, "k_out", dev)
+        if h != kh:
+            raise ValueError("k_out has k's heads")
+    a = RopeRowsArgs(n, D, qh, kh, qp, kp, qs, ks, _type(dtype), qo, ko, qos, kos, _type(otype))
+    check(lib().rkv_rope_rows(ctx.h, C.byref(rope), C.byref(a), _raw_stream(ctx, stream)))
 
 
 def append_rope(ctx: Ctx, g: Geometry, fmt: int, pages, block_tables, seq_ids, positions, k_src, v_src,
                 rope: RopeArgs | None = None, q=None, q_out=None, rule: int = Q8_CANONICAL, stream=None) -> None:
-    """Quantize-and-append into pages of format CACHE_Q8 or CACHE_MX4, keys
-    normed and rotated on the way (rope), the rows' queries beside."""
-    a = append_rope_args(fmt, seq_ids, positions, k_src, v_src, rope, q, q_out, rule)
-    if tuple(a._heads) != (g.kv_heads, g.head_dim):
-        raise ValueError("k and v rows have the geometry's heads")
-    check(lib().rkv_append_rope(ctx.h, C.byref(g), _ptr(pages), _ptr(block_tables), block_tables.shape[-1],
-                                block_tables.shape[0], C.byref(a), _stream(stream)))
+    """Quantize-and-append of rows [n][kv_heads][head_dim] (views with any row
+    stride) into pages of format CACHE_Q8 or CACHE_MX4, keys normed and rotated
+    on the way (rope); q [n][q_heads][head_dim] goes normed and rotated to q_out
+    (contiguous)."""
+    a = _append_args(ctx, g, fmt, seq_ids, positions, k_src, v_src, rope, q, q_out, rule)
+    check(lib().rkv_append_rope(ctx.h, C.byref(g), pages.data_ptr(), _i32(block_tables, "block_tables"),
+                                block_tables.shape[-1], block_tables.shape[0], C.byref(a),
+                                _raw_stream(ctx, stream)))
+
+
+def _append_args(ctx, g, fmt, seq_ids, positions, k_src, v_src, rope, q, q_out, rule) -> AppendRopeArgs:
+    n, D, dev, dtype = seq_ids.numel(), g.head_dim, ctx.device, k_src.dtype
+    kp, kh, ks = _heads(k_src, n, D, dtype, "k", dev)
+    vp, vh, vs = _heads(v_src, n, D, dtype, "v", dev)
+    if kh != g.kv_heads or vh != kh or positions.numel() != n:
+        raise ValueError("k and v rows have the geometry's heads, and a position each")
+    if rope is not None:
+        _rope_fits(rope, n, D)
+    qp, qh, qs, qo, ot = None, 0, 0, None, F32
+    if q is not None:
+        qp, qh, qs = _heads(q, n, D, dtype, "q", dev)
+        qo, h, s = _heads(q_out, n, D, q_out.dtype, "q_out", dev)
+        if h != qh or s != h * D:
+            raise ValueError("q_out: contiguous, shaped like q")
+        ot = _type(q_out.dtype)
+    return AppendRopeArgs(n, _i32(seq_ids, "seq_ids"), _i32(positions, "positions"), kp, vp, ks, vs,
+                          _type(dtype), fmt, rule, C.pointer(rope) if rope is not None else None, qp, qs, qh, qo, ot)
 
 
 def read_rows(ctx: Ctx, g: Geometry, fmt: int, pages, block_tables, seq_ids, positions, k_out, v_out,
               stream=None) -> None:
     """Values of cached rows into k_out, v_out [n][kv_heads][head_dim] (either may be None)."""
-    n = seq_ids.numel()
-    for t in (k_out, v_out):
-        if t is not None and (tuple(t.shape) != (n, g.kv_heads, g.head_dim) or not t.is_contiguous()):
+    n, kv, D, dev = seq_ids.numel(), g.kv_heads, g.head_dim, ctx.device
+    out = k_out if k_out is not None else v_out
+    if positions.numel() != n:
+        raise ValueError("one position a row")
+    at = []
+    for o in (k_out, v_out):
+        if o is None:
+            at.append(None)
+            continue
+        p, h, s = _heads(o, n, D, out.dtype, "output", dev)
+        if h != kv or s != kv * D:
             raise ValueError("outputs: contiguous [rows][kv_heads][head_dim]")
-    outs = [t for t in (k_out, v_out) if t is not None]
-    if positions.numel() != n or any(t.dtype != outs[0].dtype for t in outs):
-        raise ValueError("one position a row, outputs of one type")
-    check(lib().rkv_read_rows(ctx.h, C.byref(g), fmt, _ptr(pages), _ptr(block_tables), block_tables.shape[-1],
-                              block_tables.shape[0], n, _ptr(_i32(seq_ids, "seq_ids")),
-                              _ptr(_i32(positions, "positions")), _ptr(k_out), _ptr(v_out),
-                              _dtype(outs[0]) if outs else F32, _stream(stream)))
+        at.append(p)
+    check(lib().rkv_read_rows(ctx.h, C.byref(g), fmt, pages.data_ptr(), _i32(block_tables, "block_tables"),
+                              block_tables.shape[-1], block_tables.shape[0], n, _i32(seq_ids, "seq_ids"),
+                              _i32(positions, "positions"), *at,
+                              _type(out.dtype) if out is not None else F32, _raw_stream(ctx, stream)))
 
 
 def mx4_page_bytes(g: Geometry) -> int:
@@ -779,7 +810,7 @@ def decode_mx4(ctx: Ctx, g: Geometry, pages, block_tables, seq_lens, a: DecodeAr
     """rkv_decode_q8 over 4-bit pages (a.append must be None)."""
     check(lib().rkv_decode_mx4(ctx.h, C.byref(g), _ptr(pages), _ptr(block_tables),
                                block_tables.shape[-1], _ptr(seq_lens), seq_lens.numel(),
-                               C.byref(a), _stream(stream)))
+                               C.byref(a), _raw_stream(ctx, stream)))
 
 
 def decode_q8_partials(ctx: Ctx, g: Geometry, pages, block_tables, seq_lens, a: DecodeArgs,

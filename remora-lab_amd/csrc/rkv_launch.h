@@ -34,7 +34,8 @@ struct RopeLaunch {
   int32_t n_axes;
   const float *freqs;
   const int32_t *pair_axis;  // nullptr: axis 0
-  const int32_t *positions;  // [n_axes][n_rows]; nullptr: the appended positions
+  const int32_t *positions;  // [n_axes][n_rows]; nullptr: own
+  const int32_t *own;        // [n_rows] appended positions (nullptr: not an append)
   const void *q_norm, *k_norm;
   int32_t norm_bf16;
   float eps;

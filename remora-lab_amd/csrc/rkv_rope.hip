@@ -17,6 +17,7 @@
 // halves takes dims 4c..4c+3 and rot/2 + 4c.., so both values of its 4 pairs
 // are its own and their cosines serve every head of the row.
 #include <algorithm>
+#include <type_traits>
 
 #include "rkv_launch.h"
 #include "rkv_mx4.h"
@@ -27,6 +28,7 @@ namespace {
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef __bf16 v2b __attribute__((ext_vector_type(2)));
 
 #if defined(__HIP_DEVICE_COMPILE__)
 
@@ -99,6 +101,19 @@ __device__ __forceinline__ double dpp(double x) {
   const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), kCtrl, 0xf, 0xf, false);
   return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
+// The value of the lane 16 away, in the neighbouring row of 16: a row swap
+// leaves it in one of two registers and the lane's own in the other.
+__device__ __forceinline__ uint32_t next_row(uint32_t x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  return (threadIdx.x & 16u) ? r[0] : r[1];
+}
+__device__ __forceinline__ float next_row(float x) {
+  return __builtin_bit_cast(float, next_row(__builtin_bit_cast(uint32_t, x)));
+}
+__device__ __forceinline__ double next_row(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  return __builtin_bit_cast(double, (uint64_t)next_row((uint32_t)(u >> 32)) << 32 | next_row((uint32_t)u));
+}
 // Over kLanes (16 or 32) consecutive lanes: swaps within quads, halves of a
 // row and the row, then the neighbouring row.
 template <int kLanes, typename T>
@@ -107,7 +122,7 @@ __device__ __forceinline__ T lanes_sum(T x) {
   x += dpp<0x4e>(x);   // quad_perm 2 3 0 1
   x += dpp<0x141>(x);  // row_half_mirror
   x += dpp<0x140>(x);  // row_mirror
-  if constexpr (kLanes == 32) x += __shfl_xor(x, 16);
+  if constexpr (kLanes == 32) x += next_row(x);
   return x;
 }
 
@@ -145,7 +160,8 @@ __device__ __forceinline__ void load4(const void *src, int64_t at, bool bf16, fl
   }
 }
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
-  return (uint32_t)f32_to_bf16_rtne(a) | (uint32_t)f32_to_bf16_rtne(b) << 16;
+  const v2b r = {(__bf16)a, (__bf16)b};
+  return __builtin_bit_cast(uint32_t, r);
 }
 __device__ __forceinline__ void store4(void *out, int64_t at, bool bf16, const float (&v)[8], int from) {
   if (bf16)
@@ -166,8 +182,9 @@ __device__ __forceinline__ void load_weight(const void *w, bool bf16, const Dims
   }
 }
 
-// Norm and rotation of a head's 8 values in this lane, in T.
-template <typename T, int D>
+// Norm and rotation of a head's 8 values in this lane, in T.  kAdjacent, which
+// names the registers of a pair, is a branch of the caller's.
+template <typename T, int D, bool kAdjacent>
 __device__ __forceinline__ void turn_head(float (&v)[8], const RopeLaunch &r, bool norm, const float (&w)[8],
                                           const Turn &t, bool rotated) {
   T x[8];
@@ -185,7 +202,7 @@ __device__ __forceinline__ void turn_head(float (&v)[8], const RopeLaunch &r, bo
     T y[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int a = r.adjacent ? 2 * i : i, b = r.adjacent ? 2 * i + 1 : i + 4;
+      const int a = kAdjacent ? 2 * i : i, b = kAdjacent ? 2 * i + 1 : i + 4;
       const T c = (T)t.c[i], s = (T)t.s[i];
       y[a] = __builtin_elementwise_fma(x[a], c, -(x[b] * s));
       y[b] = __builtin_elementwise_fma(x[b], c, x[a] * s);
@@ -197,45 +214,94 @@ __device__ __forceinline__ void turn_head(float (&v)[8], const RopeLaunch &r, bo
   for (int i = 0; i < 8; ++i) v[i] = (float)x[i];
 }
 
-// Heads [h0, h1) of one row, by one wave, 512/D at a time.
-template <int D>
+// Heads [h0, h1) of one row, by one wave, 512/D at a time in batches of kBatch
+// loads; the first batch is on its way while the row's cosines are computed.
+// A pair's values, weights, cosine and sine meet in four products that are the
+// row's, so a head costs two products a value and its norm one more.
+template <int D, bool kIn16, bool kOut16, bool kAdjacent>
 __device__ __forceinline__ void turn_row(const RopeLaunch &r, const HeadRows &m, const void *weight, int64_t row,
                                          int32_t pos, int h0, int h1, int lane) {
-  constexpr int L = D / 8, kHeads = 64 / L;
+  constexpr int L = D / 8, kHeads = 64 / L, kBatch = 4;
   const int c = lane % L;
   const Dims d(r, c);
-  const bool rotated = 8 * c < r.rot_dim;
+  const bool rotated = 8 * c < r.rot_dim, norm = weight != nullptr;
+  const int64_t src = row * m.stride, dst = row * m.out_stride;
+  float v[kBatch][8];
+  auto load = [&](int first) {
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      if (first + k * kHeads >= h1) break;
+      const int h = min(first + k * kHeads + lane / L, h1 - 1);
+      load4(m.src, src + (int64_t)h * D + d.a, kIn16, v[k], 0);
+      load4(m.src, src + (int64_t)h * D + d.b, kIn16, v[k], 4);
+    }
+  };
+  load(h0);
   float w[8];
   load_weight(weight, r.norm_bf16 != 0, d, w);
-  float v[8] = {};
-  const int64_t src = row * m.stride, dst = row * m.out_stride;
-  int h = h0 + lane / L;
-  if (h < h1) {
-    load4(m.src, src + (int64_t)h * D + d.a, m.bf16 != 0, v, 0);
-    load4(m.src, src + (int64_t)h * D + d.b, m.bf16 != 0, v, 4);
-  }
-  Turn t;
-  t.load(r, row, pos, c);
-  for (int b = h0; b < h1; b += kHeads, h += kHeads) {
-    float n[8] = {};
-    if (h + kHeads < h1) {
-      load4(m.src, src + (int64_t)(h + kHeads) * D + d.a, m.bf16 != 0, n, 0);
-      load4(m.src, src + (int64_t)(h + kHeads) * D + d.b, m.bf16 != 0, n, 4);
-    }
-    turn_head<float, D>(v, r, weight != nullptr, w, t, rotated);
-    if (h < h1) {
-      store4(m.out, dst + (int64_t)h * D + d.a, m.out_bf16 != 0, v, 0);
-      store4(m.out, dst + (int64_t)h * D + d.b, m.out_bf16 != 0, v, 4);
-    }
+  // y[a] = x[a] * ca + x[b] * -sb, y[b] = x[b] * cb + x[a] * sa
+  float ca[4], cb[4], sa[4], sb[4];
+  {
+    Turn t;
+    t.load(r, row, pos, c);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = n[i];
+    for (int i = 0; i < 4; ++i) {
+      const float wa = w[kAdjacent ? 2 * i : i], wb = w[kAdjacent ? 2 * i + 1 : i + 4];
+      ca[i] = (float)t.c[i] * wa;
+      cb[i] = (float)t.c[i] * wb;
+      sa[i] = (float)t.s[i] * wa;
+      sb[i] = (float)t.s[i] * wb;
+    }
   }
+  for (int first = h0;;) {
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      if (first + k * kHeads >= h1) break;
+      const int h = first + k * kHeads + lane / L;
+      float f = 1.0f;
+      if (norm) {
+        float q = v[k][0] * v[k][0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) q = __builtin_fmaf(v[k][i], v[k][i], q);
+        f = inv_sqrt(lanes_sum<L>(q) * (1.0f / D) + r.eps);
+      }
+      float y[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int a = kAdjacent ? 2 * i : i, b = kAdjacent ? 2 * i + 1 : i + 4;
+        y[a] = v[k][a] * ca[i];
+        y[b] = v[k][b] * cb[i];
+        if (rotated) {  // (not a sine of 0: it would make NaN of an infinite partner)
+          y[a] = __builtin_fmaf(v[k][b], -sb[i], y[a]);
+          y[b] = __builtin_fmaf(v[k][a], sa[i], y[b]);
+        }
+      }
+      if (norm) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] *= f;
+      }
+      if (h < h1) {
+        store4(m.out, dst + (int64_t)h * D + d.a, kOut16, y, 0);
+        store4(m.out, dst + (int64_t)h * D + d.b, kOut16, y, 4);
+      }
+    }
+    first += kBatch * kHeads;
+    if (first >= h1) break;
+    load(first);
+  }
+}
+
+template <int D, bool kIn16, bool kOut16>
+__device__ __forceinline__ void turn_row(const RopeLaunch &r, const HeadRows &m, const void *weight, int64_t row,
+                                         int32_t pos, int h0, int h1, int lane) {
+  if (r.adjacent) turn_row<D, kIn16, kOut16, true>(r, m, weight, row, pos, h0, h1, lane);
+  else turn_row<D, kIn16, kOut16, false>(r, m, weight, row, pos, h0, h1, lane);
 }
 #endif  // __HIP_DEVICE_COMPILE__
 
 // Wave x takes head chunk x % (nq + nk) of row x / (nq + nk): nq chunks of
 // `chunk` query heads, then nk of key heads.
-template <int D>
+template <int D, bool kIn16, bool kOut16>
 __global__ __launch_bounds__(256) void rope_rows_kernel(RopeLaunch r, HeadRows q, HeadRows k, int32_t chunk) {
 #if defined(__HIP_DEVICE_COMPILE__)
   const int lane = threadIdx.x & 63;
@@ -244,8 +310,12 @@ __global__ __launch_bounds__(256) void rope_rows_kernel(RopeLaunch r, HeadRows q
   const int64_t row = x / (nq + nk);
   const int at = (int)(x % (nq + nk));
   if (row >= r.n_rows) return;
-  if (at < nq) turn_row<D>(r, q, r.q_norm, row, 0, at * chunk, min(q.heads, (at + 1) * chunk), lane);
-  else turn_row<D>(r, k, r.k_norm, row, 0, (at - nq) * chunk, min(k.heads, (at - nq + 1) * chunk), lane);
+  // (one copy of the code: the chunk's rows, heads and weight are the wave's)
+  const bool isq = at < nq;
+  const HeadRows &m = isq ? q : k;
+  const int h0 = (isq ? at : at - nq) * chunk;
+  turn_row<D, kIn16, kOut16>(r, m, isq ? r.q_norm : r.k_norm, row, r.own != nullptr ? r.own[row] : 0, h0,
+                             min(m.heads, h0 + chunk), lane);
 #endif
 }
 
@@ -328,7 +398,8 @@ __global__ __launch_bounds__(256) void append_rope_kernel(AppendRopeLaunch p, in
     const int64_t row = x / nq;
     const int at = (int)(x % nq);
     if (row < a.n_rows)
-      turn_row<D>(p.r, p.q, p.r.q_norm, row, a.positions[row], at * chunk, min(p.q.heads, (at + 1) * chunk), lane);
+      turn_row<D, kBf16, kBf16>(p.r, p.q, p.r.q_norm, row, a.positions[row], at * chunk,
+                                min(p.q.heads, (at + 1) * chunk), lane);
     return;
   }
   const int64_t row0 = (int64_t)(blockIdx.x / groups) * ROWS;
@@ -393,7 +464,8 @@ __global__ __launch_bounds__(256) void append_rope_kernel(AppendRopeLaunch p, in
       const int64_t at = (row0 + r) * p.k_stride + (int64_t)h * D;
       load4(a.k_src, at + d.a, kBf16, v, 0);
       load4(a.k_src, at + d.b, kBf16, v, 4);
-      if (p.r.on) turn_head<double, D>(v, p.r, p.r.k_norm != nullptr, w, t, rotated);
+      if (p.r.on && p.r.adjacent) turn_head<double, D, true>(v, p.r, p.r.k_norm != nullptr, w, t, rotated);
+      else if (p.r.on) turn_head<double, D, false>(v, p.r, p.r.k_norm != nullptr, w, t, rotated);
       // to 8 consecutive dims a lane, within the wave
       float *row = turned[wave][sub];
       *reinterpret_cast<v4f *>(row + d.a) = v4f{v[0], v[1], v[2], v[3]};
@@ -610,7 +682,7 @@ void launch_append_rope_r(const AppendRopeLaunch &p, hipStream_t s) {
   const uint32_t blocks = (uint32_t)(row_blocks * groups);
   uint32_t q_blocks = 0;
   int32_t chunk = 1;
-  if (p.q.src != nullptr && p.q.heads > 0) {
+  if (ROWS == 8 && p.q.src != nullptr && p.q.bf16 == p.q.out_bf16) {
     chunk = head_chunk(p.a.n_rows, p.q.heads, 512 / D);
     q_blocks = (uint32_t)(((int64_t)p.a.n_rows * ((p.q.heads + chunk - 1) / chunk) + 3) / 4);
   }
@@ -621,10 +693,18 @@ void launch_append_rope_r(const AppendRopeLaunch &p, hipStream_t s) {
     hipLaunchKernelGGL((append_rope_kernel<D, kMx4, ROWS, false>), dim3(blocks + q_blocks), dim3(256), 0, s, p, groups,
                        heads, blocks, chunk);
 }
+// 32-row workgroups once there are at least 8 per CU, else 8-row ones, which
+// take the queries into the launch: a large call's go by themselves, since the
+// append's registers leave a CU half as many of their waves (and so do those
+// of another type than the rows').
+bool small_call(const AppendRopeLaunch &p) {
+  return (int64_t)p.a.n_rows * p.a.g.kv_heads < (int64_t)32 * 8 * kComputeUnits;
+}
+bool queries_with(const AppendRopeLaunch &p) { return small_call(p) && p.q.bf16 == p.q.out_bf16; }
 template <int D, bool kMx4>
 void launch_append_rope_d(const AppendRopeLaunch &p, hipStream_t s) {
-  if ((int64_t)p.a.n_rows * p.a.g.kv_heads >= (int64_t)32 * 8 * kComputeUnits) launch_append_rope_r<D, kMx4, 32>(p, s);
-  else launch_append_rope_r<D, kMx4, 8>(p, s);
+  if (small_call(p)) launch_append_rope_r<D, kMx4, 8>(p, s);
+  else launch_append_rope_r<D, kMx4, 32>(p, s);
 }
 
 }  // namespace
@@ -635,13 +715,25 @@ hipError_t launch_rope_rows(const RopeLaunch &r, const HeadRows &q, const HeadRo
   const int32_t chunk = head_chunk(r.n_rows, q.heads + k.heads, 512 / head_dim);
   const int64_t waves = (int64_t)r.n_rows * ((q.heads + chunk - 1) / chunk + (k.heads + chunk - 1) / chunk);
   const dim3 grid((unsigned)((waves + 3) / 4));
-  if (head_dim == 256) hipLaunchKernelGGL(rope_rows_kernel<256>, grid, dim3(256), 0, s, r, q, k, chunk);
-  else hipLaunchKernelGGL(rope_rows_kernel<128>, grid, dim3(256), 0, s, r, q, k, chunk);
+  const HeadRows &m = q.heads > 0 ? q : k;
+  auto go = [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    if (m.bf16 && m.out_bf16) hipLaunchKernelGGL((rope_rows_kernel<D, true, true>), grid, dim3(256), 0, s, r, q, k, chunk);
+    else if (m.bf16) hipLaunchKernelGGL((rope_rows_kernel<D, true, false>), grid, dim3(256), 0, s, r, q, k, chunk);
+    else if (m.out_bf16) hipLaunchKernelGGL((rope_rows_kernel<D, false, true>), grid, dim3(256), 0, s, r, q, k, chunk);
+    else hipLaunchKernelGGL((rope_rows_kernel<D, false, false>), grid, dim3(256), 0, s, r, q, k, chunk);
+  };
+  if (head_dim == 256) go(std::integral_constant<int, 256>{});
+  else go(std::integral_constant<int, 128>{});
   return hipGetLastError();
 }
 
 hipError_t launch_append_rope(const AppendRopeLaunch &p, hipStream_t s) {
   if (p.a.n_rows <= 0) return hipSuccess;
+  if (p.q.src != nullptr && !queries_with(p)) {
+    const hipError_t e = launch_rope_rows(p.r, p.q, HeadRows{}, p.a.g.head_dim, s);
+    if (e != hipSuccess) return e;
+  }
   if (p.a.g.head_dim == 256) {
     if (p.mx4) launch_append_rope_d<256, true>(p, s);
     else launch_append_rope_d<256, false>(p, s);

@@ -1320,6 +1320,7 @@ rkv_status rkv_append_rope(rkv_ctx *ctx, const rkv_kv_geometry *g, void *pages, 
   l.v_stride = stride(a->v_stride, g->kv_heads);
   l.mx4 = a->format == RKV_CACHE_MX4;
   l.r = make_rope(a->rope, a->n_rows, ctx->d_fault);
+  l.r.own = a->positions;
   if (with_q)
     l.q = rkv::HeadRows{a->q_src, a->q_out, stride(a->q_stride, a->q_heads), (int64_t)a->q_heads * D, a->q_heads,
                         in16, a->q_out_dtype == RKV_BF16};

@@ -115,7 +115,7 @@ def test_binding_refuses_what_it_would_misread(rkv):
         rkv.rope_args(64, f, pos)
 
     class Ctx:
-        h = None
+        h, device = None, -1  # (a CPU tensor's device number)
     for bad in (q.half(), ):
         with pytest.raises((TypeError, ValueError)):
             rkv.rope_rows(Ctx, rope, bad, None, bad, None)
@@ -123,5 +123,14 @@ def test_binding_refuses_what_it_would_misread(rkv):
         rkv.rope_rows(Ctx, rope, torch.zeros(3, 8, 128)[:, ::2], None, q, None)
     with pytest.raises(ValueError):  # other rows than positions
         rkv.rope_rows(Ctx, rope, torch.zeros(4, 4, 128), None, torch.zeros(4, 4, 128), None)
+    class Gpu(Ctx):
+        device = 0
+    with pytest.raises(ValueError, match="device"):
+        rkv.rope_rows(Gpu, rope, q, None, q, None)
+    g = rkv.geometry(4, 128, 32, 3)
+    bt = torch.zeros(1, 1, dtype=torch.int32)
+    for k, v, sid in ((q, q[:, :2], pos), (q.double(), q.double(), pos), (q, q, pos.long()), (q, q, pos[:2])):
+        with pytest.raises((TypeError, ValueError, KeyError)):
+            rkv.append_rope(Ctx, g, rkv.CACHE_MX4, bt, bt, sid, pos, k, v, rope, stream=0)
     with pytest.raises(ValueError):
-        rkv.append_rope_args(rkv.CACHE_MX4, pos, pos, q, q[:, :2])
+        rkv.read_rows(Ctx, g, rkv.CACHE_MX4, bt, bt, pos, pos, q[:, :, :64], None, stream=0)

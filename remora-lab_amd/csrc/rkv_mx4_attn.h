@@ -8,6 +8,7 @@
 namespace rkv {
 namespace {
 
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 typedef __bf16 v2b __attribute__((ext_vector_type(2)));
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
@@ -20,14 +21,15 @@ __device__ __forceinline__ v4i load16_nt(const uint8_t *p) {
   return __builtin_nontemporal_load(reinterpret_cast<const v4i *>(p));
 }
 
-// What a wave holds of one tile.
-template <int D>
+// What a wave holds of one tile.  kScalesInLds: of the V scales only its share
+// of vmax, which the wave passes round through LDS when it needs them.
+template <int D, bool kScalesInLds = false>
 struct Mx4Tile {
   static constexpr int H = D / 128, NB = D / 32;
   v4i kc[2 * H];      // K codes of (j, h)
   uint32_t ks;        // their E8M0 bytes
   v4i vc[D / 64];     // V codes
-  v4i vs[NB / 2];     // V scale bytes of the lane's 8 tokens, 8 per block
+  v4i vs[kScalesInLds ? 1 : NB / 2];  // V scale bytes of the lane's 8 tokens, 8 per block
   uint32_t vmax;      // 2 or 4 of the tile's V scale bytes, each lane others
 
   __device__ __forceinline__ void load_k(const uint8_t *k, int lane) {
@@ -42,7 +44,7 @@ struct Mx4Tile {
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) vc[i] = load16_nt(v + 1024 * i + 16 * lane);
 #pragma unroll
-    for (int i = 0; i < NB / 2; ++i)
+    for (int i = 0; i < (kScalesInLds ? 0 : NB / 2); ++i)
       vs[i] = *reinterpret_cast<const v4i *>(v + 16 * D + 8 * NB * (lane >> 4) + 16 * i);
     if constexpr (H == 2)
       vmax = *reinterpret_cast<const uint32_t *>(v + 16 * D + 4 * lane);

@@ -30,9 +30,11 @@ template <int D, bool kTwo>
 struct Mx4Prefill {
   static constexpr int H = D / 128, NB = D / 32, G = 2;
   using Query = Mx4Query<D, false, true>;
-  using Tile = Mx4Tile<D>;
+  using Tile = Mx4Tile<D, true>;
 
-  Query q[G];
+  // the query operand of (group, half, step) at 64 lanes * 16 bytes each
+  const __attribute__((address_space(3))) v8b *q;
+  __attribute__((address_space(3))) uint8_t *vsc;  // the tile's D bytes of V scales, the wave's own
   v4f acc[G][D / 16];  // acc[2b + odd][i]: dim 32*b + 8*lg + 2*i + odd of column li
   float M[G], l[G];
   float mul;
@@ -44,18 +46,21 @@ struct Mx4Prefill {
   __device__ __forceinline__ void compute(Tile &t, int32_t tok, const uint8_t *next, uint64_t region) {
     v4f sc[G][2];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int g = 0; g < G; ++g) sc[g][0] = sc[g][1] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int g = 0; g < G; ++g) sc[g][j] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int h = 0; h < H; ++h) {
 #pragma unroll
-      for (int h = 0; h < H; ++h) {
-        const float scale = __builtin_bit_cast(float, (t.ks >> (8 * (j * H + h)) & 0xffu) << 23);
+      for (int u = 0; u < 4; ++u) {
+        v8b b[G];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int g = 0; g < G; ++g) b[g] = q[((g * H + h) * 4 + u) * 64 + lane];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float scale = __builtin_bit_cast(float, (t.ks >> (8 * (j * H + h)) & 0xffu) << 23);
           const v8b a = mx4_widen_k((uint32_t)t.kc[j * H + h][u], scale);
 #pragma unroll
           for (int g = 0; g < G; ++g)
-            sc[g][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, q[g].b[0][h][u], sc[g][j], 0, 0, 0);
+            sc[g][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[g], sc[g][j], 0, 0, 0);
         }
       }
     }
@@ -94,11 +99,18 @@ struct Mx4Prefill {
           l[g] = __builtin_amdgcn_fdot2(lo, one, l[g], false);
         }
       }
+    // every lane's word of the V scales to LDS, its group's blocks from there
+    // (a wave's LDS accesses run in order)
+    if constexpr (H == 2) *reinterpret_cast<__attribute__((address_space(3))) uint32_t *>(vsc + 4 * lane) = t.vmax;
+    else *reinterpret_cast<__attribute__((address_space(3))) uint16_t *>(vsc + 2 * lane) = (uint16_t)t.vmax;
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
     const uint32_t keep0 = mx4_keep(end - tok - 8 * lg), keep1 = mx4_keep(end - tok - 8 * lg - 4);
-    if constexpr (kMasked) drop_nan(t, tok, keep0, keep1);
+    if constexpr (kMasked) drop_nan(tok, keep0, keep1);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      uint32_t s0 = (uint32_t)t.vs[b / 2][2 * (b & 1)], s1 = (uint32_t)t.vs[b / 2][2 * (b & 1) + 1];
+      const v2u sw = scales(b);
+      uint32_t s0 = sw[0], s1 = sw[1];
       if constexpr (kMasked) {  // what lies behind the rows' tokens is nobody's
         s0 &= keep0;
         s1 &= keep1;
@@ -118,20 +130,24 @@ struct Mx4Prefill {
     if (next != nullptr) t.load_v(next + region, lane);
   }
 
+  // Bytes of the V scales of block b for the lane's 8 tokens.
+  __device__ __forceinline__ v2u scales(int b) const {
+    return *reinterpret_cast<const __attribute__((address_space(3))) v2u *>(vsc + 8 * NB * lg + 8 * b);
+  }
+
   // A masked tile with NaN V blocks: rows that attend one get NaN in its
   // dims, and the block's scale goes to 0 for the rows that do not (a weight
   // of 0 times NaN is NaN).
-  __device__ __forceinline__ void drop_nan(Tile &t, int32_t tok, uint32_t keep0, uint32_t keep1) {
+  __device__ __forceinline__ void drop_nan(int32_t tok, uint32_t keep0, uint32_t keep1) {
     auto nans = [](uint32_t s) { return ((s | 0x80808080u) - 0x7c7c7c7cu) & 0x80808080u; };  // bytes of 0x7c and more
     uint32_t any = 0;
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-      any |= nans((uint32_t)t.vs[b / 2][2 * (b & 1)] & keep0) | nans((uint32_t)t.vs[b / 2][2 * (b & 1) + 1] & keep1);
+    for (int b = 0; b < NB; ++b) any |= nans(scales(b)[0] & keep0) | nans(scales(b)[1] & keep1);
     if (__ballot(any != 0) == 0) return;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      const uint32_t s0 = (uint32_t)t.vs[b / 2][2 * (b & 1)] & keep0, s1 = (uint32_t)t.vs[b / 2][2 * (b & 1) + 1] & keep1;
-      const uint32_t n0 = nans(s0), n1 = nans(s1);
+      const v2u s = scales(b);
+      const uint32_t n0 = nans(s[0] & keep0), n1 = nans(s[1] & keep1);
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         const int32_t live = rlim[g] - tok - 8 * lg;
@@ -142,9 +158,12 @@ struct Mx4Prefill {
         acc[g][2 * b] += add;
         acc[g][2 * b + 1] += add;
       }
-      t.vs[b / 2][2 * (b & 1)] = (int32_t)(s0 & ~((n0 >> 7) * 0xffu));
-      t.vs[b / 2][2 * (b & 1) + 1] = (int32_t)(s1 & ~((n1 >> 7) * 0xffu));
+      // (every lane of the group holds and writes the same bytes)
+      *reinterpret_cast<__attribute__((address_space(3))) v2u *>(vsc + 8 * NB * lg + 8 * b) =
+          v2u{s[0] & ~((n0 >> 7) * 0xffu), s[1] & ~((n1 >> 7) * 0xffu)};
     }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
   }
 
   // A score outgrew 2^15 over its row's M: the rows' new M puts their largest
@@ -170,7 +189,7 @@ struct Mx4Prefill {
 #endif  // __HIP_DEVICE_COMPILE__
 
 template <int D, bool kTwo>
-__global__ __launch_bounds__(64 * kMx4PrefillWaves, 1) void mx4_prefill_kernel(PrefillLaunch pf) {
+__global__ __launch_bounds__(64 * kMx4PrefillWaves, 2) void mx4_prefill_kernel(PrefillLaunch pf) {
 #if defined(__HIP_DEVICE_COMPILE__)
   using Pre = Mx4Prefill<D, kTwo>;
   const DecodeLaunch &p = pf.d;
@@ -201,7 +220,11 @@ __global__ __launch_bounds__(64 * kMx4PrefillWaves, 1) void mx4_prefill_kernel(P
   const int32_t G = p.q_heads / heads;
   if (r0 / G >= jn) return;  // (waves share nothing: no barrier waits for this one)
 
+  __shared__ v8b qs[kMx4PrefillWaves][2 * 4 * Pre::H * 64];
   Pre pr;
+  __shared__ __attribute__((aligned(16))) uint8_t vscs[kMx4PrefillWaves][D];
+  pr.q = (const __attribute__((address_space(3))) v8b *)qs[r0 / 32];
+  pr.vsc = (__attribute__((address_space(3))) uint8_t *)vscs[r0 / 32];
   pr.lane = lane;
   pr.li = li;
   pr.lg = lg;
@@ -211,7 +234,10 @@ __global__ __launch_bounds__(64 * kMx4PrefillWaves, 1) void mx4_prefill_kernel(P
     const int r = r0 + 16 * c + li, jl = r / G;
     const int64_t off =
         jl < jn ? ((int64_t)(pf.qoff[e] + j0 + jl) * p.q_heads + kvh * G + r % G) * D : -1;
-    pr.q[c].load(p.q, off, p.scale_log2 < 0.0f ? -1.0f : 1.0f, false, lg);
+    typename Pre::Query q;
+    q.load(p.q, off, p.scale_log2 < 0.0f ? -1.0f : 1.0f, false, lg);
+#pragma unroll
+    for (int i = 0; i < 4 * Pre::H; ++i) qs[r0 / 32][(c * 4 * Pre::H + i) * 64 + lane] = q.b[0][i / 4][i % 4];
     pr.rlim[c] = jl < jn ? ctx + j0 + jl + 1 : 0;
     pr.M[c] = kNoMax;
     pr.l[c] = 0.0f;
@@ -240,10 +266,16 @@ __global__ __launch_bounds__(64 * kMx4PrefillWaves, 1) void mx4_prefill_kernel(P
     const uint8_t *at = place(tok0);
     t.load_k(at, lane);
     t.load_v(at + RB, lane);
-    for (int32_t tok = tok0; tok < last; tok += kTile) {
+    // two loops and not one with a choice: each keeps the sums in place
+    int32_t tok = tok0;
+    const int32_t whole = min(all, last);
+    for (; tok + kTile <= whole; tok += kTile) {
       at = tok + kTile < last ? place(tok + kTile) : nullptr;
-      if (tok + kTile > min(all, last)) pr.template compute<true>(t, tok, at, RB);
-      else pr.template compute<false>(t, tok, at, RB);
+      pr.template compute<false>(t, tok, at, RB);
+    }
+    for (; tok < last; tok += kTile) {
+      at = tok + kTile < last ? place(tok + kTile) : nullptr;
+      pr.template compute<true>(t, tok, at, RB);
     }
   }
   if (bad && lane == 0) atomicOr(p.fault, FAULT_BAD_PAGE);
@@ -269,11 +301,10 @@ __global__ __launch_bounds__(64 * kMx4PrefillWaves, 1) void mx4_prefill_kernel(P
         *reinterpret_cast<v4f *>(pf.ws_o + prow * D + d0) = o0;
         *reinterpret_cast<v4f *>(pf.ws_o + prow * D + d0 + 4) = o1;
       } else if (p.out_bf16 != 0) {
-        uint32_t w[4];
+        v8b w;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          w[i] = (uint32_t)f32_to_bf16_rtne(ev[i]) | (uint32_t)f32_to_bf16_rtne(od[i]) << 16;
-        *reinterpret_cast<v4u *>(static_cast<uint16_t *>(p.out) + orow * D + d0) = v4u{w[0], w[1], w[2], w[3]};
+        for (int i = 0; i < 8; ++i) w[i] = (__bf16)(i & 1 ? od[i / 2] : ev[i / 2]);
+        *reinterpret_cast<v8b *>(static_cast<uint16_t *>(p.out) + orow * D + d0) = w;
       } else {
         *reinterpret_cast<v4f *>(static_cast<float *>(p.out) + orow * D + d0) = o0;
         *reinterpret_cast<v4f *>(static_cast<float *>(p.out) + orow * D + d0 + 4) = o1;

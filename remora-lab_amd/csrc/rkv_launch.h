@@ -155,9 +155,8 @@ hipError_t launch_decode(const DecodeLaunch &d, hipStream_t s);
 // 32, pt_unit one tile of every wave, and a partition may span any pages.
 // append, the per-entry partials layout and the LDS ring depth have no part in it.
 constexpr int kMx4Waves = 4;
-// Workgroups resident per CU: two waves a SIMD up to 16 rows per kv head (8
-// with an f32 query, which takes three times the registers), one above.
-constexpr int mx4_wgs_per_cu(int rows, bool q_bf16) { return rows > (q_bf16 ? 16 : 8) ? 1 : 2; }
+// Workgroups resident per CU: two waves a SIMD (up to 256 registers a lane).
+constexpr int kMx4WgsPerCu = 2;
 hipError_t launch_mx4_decode(const DecodeLaunch &d, hipStream_t s);
 
 // Chunked prefill attention: entry e holds rows[e] query rows of sequence

@@ -25,180 +25,16 @@ namespace {
 
 constexpr int kMx4PrefillWaves = 4;
 
-#if defined(__HIP_DEVICE_COMPILE__)
-template <int D, bool kTwo>
-struct Mx4Prefill {
-  static constexpr int H = D / 128, NB = D / 32, G = 2;
-  using Query = Mx4Query<D, false, true>;
-  using Tile = Mx4Tile<D, true>;
-
-  // the query operand of (group, half, step) at 64 lanes * 16 bytes each
-  const __attribute__((address_space(3))) v8b *q;
-  __attribute__((address_space(3))) uint8_t *vsc;  // the tile's D bytes of V scales, the wave's own
-  v4f acc[G][D / 16];  // acc[2b + odd][i]: dim 32*b + 8*lg + 2*i + odd of column li
-  float M[G], l[G];
-  float mul;
-  int32_t rlim[G];     // positions that the lane's row attends
-  int32_t end;         // positions that any of the wave's rows attends
-  int lane, li, lg;
-
-  template <bool kMasked>
-  __device__ __forceinline__ void compute(Tile &t, int32_t tok, const uint8_t *next, uint64_t region) {
-    v4f sc[G][2];
-#pragma unroll
-    for (int g = 0; g < G; ++g) sc[g][0] = sc[g][1] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int h = 0; h < H; ++h) {
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        v8b b[G];
-#pragma unroll
-        for (int g = 0; g < G; ++g) b[g] = q[((g * H + h) * 4 + u) * 64 + lane];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float scale = __builtin_bit_cast(float, (t.ks >> (8 * (j * H + h)) & 0xffu) << 23);
-          const v8b a = mx4_widen_k((uint32_t)t.kc[j * H + h][u], scale);
-#pragma unroll
-          for (int g = 0; g < G; ++g)
-            sc[g][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[g], sc[g][j], 0, 0, 0);
-        }
-      }
-    }
-    if (next != nullptr) t.load_k(next, lane);
-    v8h w[G][kTwo ? 2 : 1];
-    float x[G][8];
-    bool high = false;
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-      const int32_t live = rlim[g] - tok - 8 * lg;
-      float top = kNoMax;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[g][i] = sc[g][i / 4][i % 4];
-        if constexpr (kMasked) x[g][i] = i < live ? x[g][i] : -INFINITY;
-        top = fmaxf(top, x[g][i]);
-      }
-      high = high || __builtin_fmaf(top, mul, -M[g]) > 15.0f;
-    }
-    if (__ballot(high) != 0) rescale(x);
-    const v2h one = {(_Float16)1.0f, (_Float16)1.0f};
-#pragma unroll
-    for (int g = 0; g < G; ++g)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[g][2 * i], mul, -M[g]));
-        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[g][2 * i + 1], mul, -M[g]));
-        const v2h hi = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(p0, p1));
-        w[g][0][2 * i] = hi[0];
-        w[g][0][2 * i + 1] = hi[1];
-        l[g] = __builtin_amdgcn_fdot2(hi, one, l[g], false);
-        if constexpr (kTwo) {
-          const v2h lo = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(p0 - (float)hi[0], p1 - (float)hi[1]));
-          w[g][1][2 * i] = lo[0];
-          w[g][1][2 * i + 1] = lo[1];
-          l[g] = __builtin_amdgcn_fdot2(lo, one, l[g], false);
-        }
-      }
-    // every lane's word of the V scales to LDS, its group's blocks from there
-    // (a wave's LDS accesses run in order)
-    if constexpr (H == 2) *reinterpret_cast<__attribute__((address_space(3))) uint32_t *>(vsc + 4 * lane) = t.vmax;
-    else *reinterpret_cast<__attribute__((address_space(3))) uint16_t *>(vsc + 2 * lane) = (uint16_t)t.vmax;
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    const uint32_t keep0 = mx4_keep(end - tok - 8 * lg), keep1 = mx4_keep(end - tok - 8 * lg - 4);
-    if constexpr (kMasked) drop_nan(tok, keep0, keep1);
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const v2u sw = scales(b);
-      uint32_t s0 = sw[0], s1 = sw[1];
-      if constexpr (kMasked) {  // what lies behind the rows' tokens is nobody's
-        s0 &= keep0;
-        s1 &= keep1;
-      }
-      const v8h m = mx4_v_scales(s0, s1);
-#pragma unroll
-      for (int odd = 0; odd < 2; ++odd) {
-        const int dt = 2 * b + odd;
-        const v8h a = mx4_widen_v((uint32_t)t.vc[dt / 4][dt % 4], 0x1p-2f) * m;  // V times 2^6
-#pragma unroll
-        for (int g = 0; g < G; ++g)
-#pragma unroll
-          for (int k = 0; k < (kTwo ? 2 : 1); ++k)
-            acc[g][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, w[g][k], acc[g][dt], 0, 0, 0);
-      }
-    }
-    if (next != nullptr) t.load_v(next + region, lane);
-  }
-
-  // Bytes of the V scales of block b for the lane's 8 tokens.
-  __device__ __forceinline__ v2u scales(int b) const {
-    return *reinterpret_cast<const __attribute__((address_space(3))) v2u *>(vsc + 8 * NB * lg + 8 * b);
-  }
-
-  // A masked tile with NaN V blocks: rows that attend one get NaN in its
-  // dims, and the block's scale goes to 0 for the rows that do not (a weight
-  // of 0 times NaN is NaN).
-  __device__ __forceinline__ void drop_nan(int32_t tok, uint32_t keep0, uint32_t keep1) {
-    auto nans = [](uint32_t s) { return ((s | 0x80808080u) - 0x7c7c7c7cu) & 0x80808080u; };  // bytes of 0x7c and more
-    uint32_t any = 0;
-#pragma unroll
-    for (int b = 0; b < NB; ++b) any |= nans(scales(b)[0] & keep0) | nans(scales(b)[1] & keep1);
-    if (__ballot(any != 0) == 0) return;
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const v2u s = scales(b);
-      const uint32_t n0 = nans(s[0] & keep0), n1 = nans(s[1] & keep1);
-#pragma unroll
-      for (int g = 0; g < G; ++g) {
-        const int32_t live = rlim[g] - tok - 8 * lg;
-        int hit = ((n0 & mx4_keep(live)) | (n1 & mx4_keep(live - 4))) != 0u;
-        hit |= __shfl_xor(hit, 16);
-        hit |= __shfl_xor(hit, 32);
-        const float add = hit ? __builtin_nanf("") : 0.0f;
-        acc[g][2 * b] += add;
-        acc[g][2 * b + 1] += add;
-      }
-      // (every lane of the group holds and writes the same bytes)
-      *reinterpret_cast<__attribute__((address_space(3))) v2u *>(vsc + 8 * NB * lg + 8 * b) =
-          v2u{s[0] & ~((n0 >> 7) * 0xffu), s[1] & ~((n1 >> 7) * 0xffu)};
-    }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-  }
-
-  // A score outgrew 2^15 over its row's M: the rows' new M puts their largest
-  // at 2^11, and the sums go into its units.
-  __device__ __forceinline__ void rescale(const float (&x)[G][8]) {
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-      float top = x[g][0];
-#pragma unroll
-      for (int i = 1; i < 8; ++i) top = fmaxf(top, x[g][i]);
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
-      float n = __builtin_fmaf(top, mul, -11.0f);
-      if (!(n > M[g])) n = M[g];
-      const float f = __builtin_amdgcn_exp2f(M[g] - n);
-      M[g] = n;
-      l[g] *= f;
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) acc[g][i] *= f;
-    }
-  }
-};
-#endif  // __HIP_DEVICE_COMPILE__
-
 template <int D, bool kTwo>
 __global__ __launch_bounds__(64 * kMx4PrefillWaves, 2) void mx4_prefill_kernel(PrefillLaunch pf) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  using Pre = Mx4Prefill<D, kTwo>;
+  using Pre = Mx4Wide<D, 2, kTwo, true>;
   const DecodeLaunch &p = pf.d;
-  const Geo g = p.g;
   // the workgroup's unit (see prefill_kernel)
   const uint32_t C = (uint32_t)max(pf.xcd_chunk, 1);
   const uint32_t xcd = blockIdx.x & 7u, slot = blockIdx.x >> 3;
   const int64_t x = ((int64_t)xcd + 8 * (int64_t)(slot / C)) * C + slot % C;
-  const int32_t heads = g.kv_heads;
+  const int32_t heads = p.g.kv_heads;
   if (x >= (int64_t)pf.first[pf.n_entries] * heads) return;
   int e = 0;
   while (e + 1 < pf.n_entries && x >= (int64_t)pf.first[e + 1] * heads) ++e;
@@ -220,7 +56,7 @@ __global__ __launch_bounds__(64 * kMx4PrefillWaves, 2) void mx4_prefill_kernel(P
   const int32_t G = p.q_heads / heads;
   if (r0 / G >= jn) return;  // (waves share nothing: no barrier waits for this one)
 
-  __shared__ v8b qs[kMx4PrefillWaves][2 * 4 * Pre::H * 64];
+  __shared__ v8b qs[kMx4PrefillWaves][Pre::kQuery];
   Pre pr;
   __shared__ __attribute__((aligned(16))) uint8_t vscs[kMx4PrefillWaves][D];
   pr.q = (const __attribute__((address_space(3))) v8b *)qs[r0 / 32];
@@ -234,10 +70,7 @@ __global__ __launch_bounds__(64 * kMx4PrefillWaves, 2) void mx4_prefill_kernel(P
     const int r = r0 + 16 * c + li, jl = r / G;
     const int64_t off =
         jl < jn ? ((int64_t)(pf.qoff[e] + j0 + jl) * p.q_heads + kvh * G + r % G) * D : -1;
-    typename Pre::Query q;
-    q.load(p.q, off, p.scale_log2 < 0.0f ? -1.0f : 1.0f, false, lg);
-#pragma unroll
-    for (int i = 0; i < 4 * Pre::H; ++i) qs[r0 / 32][(c * 4 * Pre::H + i) * 64 + lane] = q.b[0][i / 4][i % 4];
+    pr.put_query(qs[r0 / 32], c, p.q, off, p.scale_log2 < 0.0f ? -1.0f : 1.0f);
     pr.rlim[c] = jl < jn ? ctx + j0 + jl + 1 : 0;
     pr.M[c] = kNoMax;
     pr.l[c] = 0.0f;
@@ -249,36 +82,9 @@ __global__ __launch_bounds__(64 * kMx4PrefillWaves, 2) void mx4_prefill_kernel(P
   pr.end = ctx + j0 + min((r0 + 31) / G, jn - 1) + 1;
   const int32_t last = min(tok_end, pr.end);
 
-  const uint64_t PB = mx4_page_bytes(g), RB = mx4_region_bytes(g);
-  const uint8_t *base = p.pages + (uint64_t)kvh * 2u * RB;
-  const int32_t *bt = p.bt + (int64_t)seq * p.bt_stride;
-  bool bad = false;
-  auto place = [&](int32_t tok) -> const uint8_t * {
-    int32_t page = bt[tok / g.page_tokens];
-    if (page < 0 || page >= g.num_pages) {
-      bad = true;
-      page = 0;
-    }
-    return base + (uint64_t)page * PB + (uint64_t)(tok % g.page_tokens / kTile) * mx4_tile_bytes(D);
-  };
-  typename Pre::Tile t;
-  if (tok0 < last) {
-    const uint8_t *at = place(tok0);
-    t.load_k(at, lane);
-    t.load_v(at + RB, lane);
-    // two loops and not one with a choice: each keeps the sums in place
-    int32_t tok = tok0;
-    const int32_t whole = min(all, last);
-    for (; tok + kTile <= whole; tok += kTile) {
-      at = tok + kTile < last ? place(tok + kTile) : nullptr;
-      pr.template compute<false>(t, tok, at, RB);
-    }
-    for (; tok < last; tok += kTile) {
-      at = tok + kTile < last ? place(tok + kTile) : nullptr;
-      pr.template compute<true>(t, tok, at, RB);
-    }
-  }
-  if (bad && lane == 0) atomicOr(p.fault, FAULT_BAD_PAGE);
+  Mx4Place at(p, seq, kvh);
+  mx4_walk<D>(pr, at, tok0, kTile, min(all, last), last);
+  if (at.bad && lane == 0) atomicOr(p.fault, FAULT_BAD_PAGE);
 
 #pragma unroll
   for (int c = 0; c < 2; ++c) {

@@ -646,8 +646,7 @@ Plan mx4_plan_of(const rkv_kv_geometry *g, const rkv_decode_args *a) {
   Plan pl;
   pl.unit = 32 * rkv::kMx4Waves;
   pl.max_len = std::max<int32_t>(a->max_seq_len, 1);
-  const int32_t rows = a->q_len * (a->q_heads / g->kv_heads);
-  pl.target = std::max(1, rkv::kComputeUnits * rkv::mx4_wgs_per_cu(rows, a->q_dtype == RKV_BF16) / g->kv_heads);
+  pl.target = std::max(1, rkv::kComputeUnits * rkv::kMx4WgsPerCu / g->kv_heads);
   const int64_t B = std::max<int32_t>(a->batch, 0);
   const int32_t rounds = (pl.max_len + pl.unit - 1) / pl.unit;
   pl.kmin = rounds <= kMx4Whole ? rounds : 1;

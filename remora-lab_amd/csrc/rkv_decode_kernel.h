@@ -1913,8 +1913,15 @@ __device__ __forceinline__ bool locate(const DecodeLaunch &p, int lane, int32_t 
     }
     const int32_t k0 = (units + p.target_parts - 1) / p.target_parts;
     int32_t lo = max(p.pt_kmin, min(k0, p.pt_kmax)), hi = p.pt_kmax;
+    // and count(k*unit) <= (that sum) / k + batch, so k = sum / (target -
+    // batch) will do: with many more partitions than entries the two ends
+    // are next to each other
+    const int32_t spare = p.target_parts - p.batch;
+    const int32_t enough = spare > 0 ? (units + spare - 1) / spare : p.pt_kmax;
+    const bool known = spare > 0 && enough <= hi;
+    if (known) hi = max(lo, enough);
     if (count(len_of(lo)) > p.target_parts) {
-      if (count(len_of(hi)) > p.target_parts) {
+      if (!known && count(len_of(hi)) > p.target_parts) {
         lo = hi;
       } else {
         ++lo;

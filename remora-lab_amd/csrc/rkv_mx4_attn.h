@@ -155,16 +155,20 @@ struct Mx4Place {
   }
 };
 
-// A wave's walk over the tiles at tok0, tok0 + step, .. below `end`, those
-// that end at or before `whole` unmasked.  (Two loops and not one with a
-// choice: each keeps the sums in place.)
-template <int D, typename Work>
-__device__ __forceinline__ void mx4_walk(Work &w, Mx4Place &at, int32_t tok, int32_t step, int32_t whole, int32_t end) {
-  if (tok >= end) return;
+// A wave's walk over the tiles at tok, tok + step, .. below `end`, those that
+// end at or before `whole` unmasked.  `ready` runs when the first tile's loads
+// are on their way.  (Two loops and not one with a choice: each keeps the sums
+// in place.)
+template <int D, typename Work, typename Ready>
+__device__ __forceinline__ void mx4_walk(Work &w, Mx4Place &at, int32_t tok, int32_t step, int32_t whole, int32_t end,
+                                         Ready ready) {
   typename Work::Tile t;
-  const uint8_t *k = at.tile<D>(tok);
-  t.load_k(k, w.lane);
-  t.load_v(k + at.region, w.lane);
+  if (tok < end) {
+    const uint8_t *k = at.tile<D>(tok);
+    t.load_k(k, w.lane);
+    t.load_v(k + at.region, w.lane);
+  }
+  ready();
   for (; tok + kTile <= whole && tok < end; tok += step)
     w.template compute<false>(t, tok, tok + step < end ? at.tile<D>(tok + step) : nullptr, at.region);
   for (; tok < end; tok += step)

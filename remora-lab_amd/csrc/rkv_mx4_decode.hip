@@ -254,7 +254,6 @@ __global__ __launch_bounds__(64 * NW, 2) void mx4_decode_kernel(DecodeLaunch p) 
   dc.losel = li >= 8 ? -1.0f : 0.0f;
   dc.end = part.tok_end;
   const int64_t row = query_row(p, part.b, kvh, li & 7);
-  dc.q.load(p.q, row < 0 ? -1 : row * D, p.scale_log2 < 0.0f ? -1.0f : 1.0f, li >= 8, lg);
   dc.rlim = row < 0 ? 0 : part.len - p.q_len + (li & 7) / G + 1;
   dc.M = kNoMax;
   dc.l = 0.0f;
@@ -263,7 +262,8 @@ __global__ __launch_bounds__(64 * NW, 2) void mx4_decode_kernel(DecodeLaunch p) 
 
   // the wave's tiles: tok0 + 32*wave, then every NW-th; row 0 attends len - q_len + 1 positions
   Mx4Place at(p, part.seq, kvh);
-  mx4_walk<D>(dc, at, part.tok0 + kTile * wave, kTile * NW, min(part.len - p.q_len + 1, part.tok_end), part.tok_end);
+  mx4_walk<D>(dc, at, part.tok0 + kTile * wave, kTile * NW, min(part.len - p.q_len + 1, part.tok_end), part.tok_end,
+              [&] { dc.q.load(p.q, row < 0 ? -1 : row * D, p.scale_log2 < 0.0f ? -1.0f : 1.0f, li >= 8, lg); });
   if (at.bad && lane == 0) atomicOr(p.fault, FAULT_BAD_PAGE);
 
   // ---- merge of the waves: second terms onto the first, then every wave's rows side by side
@@ -328,18 +328,20 @@ __global__ __launch_bounds__(64 * NW, 2) void mx4_decode_wide_kernel(DecodeLaunc
   dc.end = part.tok_end;
 #pragma unroll
   for (int c = 0; c < G; ++c) {
-    const int64_t row = query_row(p, part.b, kvh, 16 * c + li);
-    if (wave == c)
-      dc.put_query(reinterpret_cast<v8b *>(shared), c, p.q, row < 0 ? -1 : row * D, p.scale_log2 < 0.0f ? -1.0f : 1.0f);
-    dc.rlim[c] = row < 0 ? 0 : part.len - p.q_len + (16 * c + li) / heads + 1;
+    dc.rlim[c] = 16 * c + li >= R ? 0 : part.len - p.q_len + (16 * c + li) / heads + 1;
     dc.M[c] = kNoMax;
     dc.l[c] = 0.0f;
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) dc.acc[c][i] = v4f{0.f, 0.f, 0.f, 0.f};
   }
-  __syncthreads();
   Mx4Place at(p, part.seq, kvh);
-  mx4_walk<D>(dc, at, part.tok0 + kTile * wave, kTile * NW, min(part.len - p.q_len + 1, part.tok_end), part.tok_end);
+  mx4_walk<D>(dc, at, part.tok0 + kTile * wave, kTile * NW, min(part.len - p.q_len + 1, part.tok_end), part.tok_end, [&] {
+    if (wave < G) {
+      const int64_t row = query_row(p, part.b, kvh, 16 * wave + li);
+      dc.put_query(reinterpret_cast<v8b *>(shared), wave, p.q, row < 0 ? -1 : row * D, p.scale_log2 < 0.0f ? -1.0f : 1.0f);
+    }
+    __syncthreads();
+  });
   if (at.bad && lane == 0) atomicOr(p.fault, FAULT_BAD_PAGE);
 
 #pragma unroll

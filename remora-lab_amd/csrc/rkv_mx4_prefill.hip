@@ -83,7 +83,7 @@ __global__ __launch_bounds__(64 * kMx4PrefillWaves, 2) void mx4_prefill_kernel(P
   const int32_t last = min(tok_end, pr.end);
 
   Mx4Place at(p, seq, kvh);
-  mx4_walk<D>(pr, at, tok0, kTile, min(all, last), last);
+  mx4_walk<D>(pr, at, tok0, kTile, min(all, last), last, [] {});
   if (at.bad && lane == 0) atomicOr(p.fault, FAULT_BAD_PAGE);
 
 #pragma unroll

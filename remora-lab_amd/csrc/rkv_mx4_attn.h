@@ -21,16 +21,16 @@ __device__ __forceinline__ v4i load16_nt(const uint8_t *p) {
   return __builtin_nontemporal_load(reinterpret_cast<const v4i *>(p));
 }
 
-// What a wave holds of one tile.  kScalesInLds: of the V scales only its share
-// of vmax, which the wave passes round through LDS when it needs them.
-template <int D, bool kScalesInLds = false>
+// What a wave holds of one tile.  Of the V scales each lane has others, which
+// the wave passes round through LDS when it needs them (loaded by every lane
+// that needs them they would take 16 registers and four loads more).
+template <int D>
 struct Mx4Tile {
   static constexpr int H = D / 128, NB = D / 32;
   v4i kc[2 * H];      // K codes of (j, h)
   uint32_t ks;        // their E8M0 bytes
   v4i vc[D / 64];     // V codes
-  v4i vs[kScalesInLds ? 1 : NB / 2];  // V scale bytes of the lane's 8 tokens, 8 per block
-  uint32_t vmax;      // 2 or 4 of the tile's V scale bytes, each lane others
+  uint32_t vsw;       // 4 (D 128: 2) of the tile's V scale bytes
 
   __device__ __forceinline__ void load_k(const uint8_t *k, int lane) {
 #pragma unroll
@@ -43,13 +43,10 @@ struct Mx4Tile {
   __device__ __forceinline__ void load_v(const uint8_t *v, int lane) {
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) vc[i] = load16_nt(v + 1024 * i + 16 * lane);
-#pragma unroll
-    for (int i = 0; i < (kScalesInLds ? 0 : NB / 2); ++i)
-      vs[i] = *reinterpret_cast<const v4i *>(v + 16 * D + 8 * NB * (lane >> 4) + 16 * i);
     if constexpr (H == 2)
-      vmax = *reinterpret_cast<const uint32_t *>(v + 16 * D + 4 * lane);
+      vsw = *reinterpret_cast<const uint32_t *>(v + 16 * D + 4 * lane);
     else
-      vmax = *reinterpret_cast<const uint16_t *>(v + 16 * D + 2 * lane);
+      vsw = *reinterpret_cast<const uint16_t *>(v + 16 * D + 2 * lane);
   }
 };
 
@@ -131,6 +128,21 @@ __device__ __forceinline__ v8h mx4_v_scales(uint32_t s0, uint32_t s1) {
 // Bytes of a word of scales that belong to the first n of its 4 tokens.
 __device__ __forceinline__ uint32_t mx4_keep(int32_t n) { return n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1u; }
 
+// A tile's V scales in LDS, the wave's own D bytes: every lane's word in (a
+// wave's LDS accesses run in order), and the bytes of block b for the 8 tokens
+// of a lane's group out.
+template <int D>
+__device__ __forceinline__ void mx4_put_scales(__attribute__((address_space(3))) uint8_t *vsc, uint32_t w, int lane) {
+  if constexpr (D == 256) *reinterpret_cast<__attribute__((address_space(3))) uint32_t *>(vsc + 4 * lane) = w;
+  else *reinterpret_cast<__attribute__((address_space(3))) uint16_t *>(vsc + 2 * lane) = (uint16_t)w;
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+template <int D>
+__device__ __forceinline__ v2u mx4_get_scales(const __attribute__((address_space(3))) uint8_t *vsc, int b, int lg) {
+  return *reinterpret_cast<const __attribute__((address_space(3))) v2u *>(vsc + D / 4 * lg + 8 * b);
+}
+
 // A kv head's tiles of one sequence.  A page id outside the pool reads page 0
 // and is remembered.
 struct Mx4Place {
@@ -182,7 +194,7 @@ struct Mx4Wide {
   static constexpr int H = D / 128, NB = D / 32;
   using Query = Mx4Query<D, false, kBf16>;
   static constexpr int kQuery = G * H * 4 * Query::kSets * 64;  // the query operand's 16-byte words in LDS
-  using Tile = Mx4Tile<D, true>;
+  using Tile = Mx4Tile<D>;
 
   // the query operand of (group, half, step, term), 64 lanes' words each
   const __attribute__((address_space(3))) v8b *q;
@@ -268,12 +280,7 @@ struct Mx4Wide {
           l[g] = __builtin_amdgcn_fdot2(lo, one, l[g], false);
         }
       }
-    // every lane's word of the V scales to LDS, its group's blocks from there
-    // (a wave's LDS accesses run in order)
-    if constexpr (H == 2) *reinterpret_cast<__attribute__((address_space(3))) uint32_t *>(vsc + 4 * lane) = t.vmax;
-    else *reinterpret_cast<__attribute__((address_space(3))) uint16_t *>(vsc + 2 * lane) = (uint16_t)t.vmax;
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+    mx4_put_scales<D>(vsc, t.vsw, lane);
     const uint32_t keep0 = mx4_keep(end - tok - 8 * lg), keep1 = mx4_keep(end - tok - 8 * lg - 4);
     if constexpr (kMasked) drop_nan(tok, keep0, keep1);
 #pragma unroll
@@ -299,10 +306,7 @@ struct Mx4Wide {
     if (next != nullptr) t.load_v(next + region, lane);
   }
 
-  // Bytes of the V scales of block b for the lane's 8 tokens.
-  __device__ __forceinline__ v2u scales(int b) const {
-    return *reinterpret_cast<const __attribute__((address_space(3))) v2u *>(vsc + 8 * NB * lg + 8 * b);
-  }
+  __device__ __forceinline__ v2u scales(int b) const { return mx4_get_scales<D>(vsc, b, lg); }
 
   // A masked tile with NaN V blocks: rows that attend one get NaN in its
   // dims, and the block's scale goes to 0 for the rows that do not (a weight

@@ -44,6 +44,7 @@ struct Mx4Narrow {
   using Tile = Mx4Tile<D>;
 
   Query q;
+  __attribute__((address_space(3))) uint8_t *vsc;  // the tile's D bytes of V scales, the wave's own
   v4f acc[D / 16];  // acc[2b + odd][i]: dim 32*b + 8*lg + 2*i + odd of column li
   float M, l;
   float mul;        // |scale| * log2 e
@@ -83,7 +84,7 @@ struct Mx4Narrow {
       if constexpr (kMasked) x[i] = i < live ? x[i] : -INFINITY;
     }
     // s - M of the largest score, and the V scales against vcap
-    const uint32_t vmax = kMasked ? t.vmax & vlive(end - tok) : t.vmax;
+    const uint32_t vmax = kMasked ? t.vsw & vlive(end - tok) : t.vsw;
     const uint32_t cap = (uint32_t)(4 * (vcap + 15)) * 0x01010101u;
     float top = x[0];
 #pragma unroll
@@ -104,11 +105,13 @@ struct Mx4Narrow {
       w[2 * i + 1] = own[1];
       l = __builtin_amdgcn_fdot2(own, one, l, false);
     }
+    mx4_put_scales<D>(vsc, t.vsw, lane);
     // masked tiles: the row's own tokens' scales only (a weight of 0 times NaN is NaN)
     const uint32_t keep0 = mx4_keep(live), keep1 = mx4_keep(live - 4);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      uint32_t s0 = (uint32_t)t.vs[b / 2][2 * (b & 1)], s1 = (uint32_t)t.vs[b / 2][2 * (b & 1) + 1];
+      const v2u sw = mx4_get_scales<D>(vsc, b, lg);
+      uint32_t s0 = sw[0], s1 = sw[1];
       if constexpr (kMasked) {
         s0 &= keep0;
         s1 &= keep1;
@@ -124,7 +127,7 @@ struct Mx4Narrow {
     if (next != nullptr) t.load_v(next + region, lane);
   }
 
-  // The bytes of vmax that belong to the tile's first n tokens: what a page
+  // The bytes of vsw that belong to the tile's first n tokens: what a page
   // holds behind them is nobody's, and no result may follow it.
   __device__ __forceinline__ uint32_t vlive(int32_t n) const {
     constexpr int kPer = H == 2 ? 4 : 2;  // tokens of a lane, of group lane / 16
@@ -232,12 +235,13 @@ __device__ __forceinline__ void put_sums(float *dst, const v4f *acc, int lg, flo
 #endif  // __HIP_DEVICE_COMPILE__
 
 template <int D, bool kBf16, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void mx4_decode_kernel(DecodeLaunch p) {
+__global__ __launch_bounds__(64 * NW, kMx4WgsPerCu) void mx4_decode_kernel(DecodeLaunch p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   using Dec = Mx4Narrow<D, kBf16>;
   constexpr int kStride = D + 4;  // floats between a row's sums in LDS
   __shared__ __attribute__((aligned(16))) float sums[NW][8][kStride];
   __shared__ float ms[NW][8], ls[NW][8];
+  __shared__ __attribute__((aligned(16))) uint8_t vscs[NW][D];
   Dec dc;
   const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
   const int wave = (int)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -250,6 +254,7 @@ __global__ __launch_bounds__(64 * NW, 2) void mx4_decode_kernel(DecodeLaunch p) 
   const int32_t G = p.q_heads / p.g.kv_heads, R = p.q_len * G;
   // at least the smallest normal: a masked -inf times it stays -inf with a scale of 0
   dc.mul = fmaxf(fabsf(p.scale_log2), 1.17549435e-38f);
+  dc.vsc = (__attribute__((address_space(3))) uint8_t *)vscs[wave];
   dc.vcap = 0;
   dc.losel = li >= 8 ? -1.0f : 0.0f;
   dc.end = part.tok_end;
@@ -304,7 +309,7 @@ __global__ __launch_bounds__(64 * NW, 2) void mx4_decode_kernel(DecodeLaunch p) 
 // G groups of 16 rows.  The query (and, when the waves are done with it, the
 // rows' sums, wave after wave) is the workgroup's.
 template <int D, int G, bool kBf16, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void mx4_decode_wide_kernel(DecodeLaunch p) {
+__global__ __launch_bounds__(64 * NW, kMx4WgsPerCu) void mx4_decode_wide_kernel(DecodeLaunch p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   using Dec = Mx4Wide<D, G, true, kBf16>;  // (weights of two terms cost a verify of 32 x 32k rows 1 us of 152)
   constexpr int kStride = D + 4;

@@ -27,6 +27,7 @@ namespace {
 
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef float v2f __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef __bf16 v2b __attribute__((ext_vector_type(2)));
 
@@ -66,25 +67,34 @@ __device__ __forceinline__ void sin_cos(double a, double &s, double &c) {
   c = (q + 1) & 2 ? -c : c;
 }
 
-// Cosines and sines of lane c's 4 pairs of a row (1 and 0 past the rotated dims).
+// The angle of a pair, from the row's positions on the axes.
+__device__ __forceinline__ double angle(const RopeLaunch &r, int pair, const int32_t (&at)[4]) {
+  int32_t axis = r.pair_axis != nullptr ? r.pair_axis[pair] : 0;
+  if (axis < 0 || axis >= r.n_axes) {
+    atomicOr(r.fault, FAULT_BAD_POSITION);
+    axis = 0;
+  }
+  return (double)(axis == 0 ? at[0] : axis == 1 ? at[1] : axis == 2 ? at[2] : at[3]) * (double)r.freqs[pair];
+}
+
+// Cosines and sines of lane c's 4 pairs of a row (1 and 0 past the rotated
+// dims).  The loads of a row are independent of each other: its positions on
+// every axis, and the axes that choose among them.
 struct Turn {
   double c[4], s[4];
   __device__ __forceinline__ void load(const RopeLaunch &r, int64_t row, int32_t pos, int lane) {
-    const bool in = 8 * lane < r.rot_dim;
+    int32_t at[4] = {pos, pos, pos, pos};
+    if (r.positions != nullptr)
+#pragma unroll
+      for (int a = 0; a < 4; ++a) at[a] = r.positions[(int64_t)min(a, r.n_axes - 1) * r.n_rows + row];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       c[i] = 1.0;
       s[i] = 0.0;
-      if (!in) continue;
-      const int pair = 4 * lane + i;
-      int32_t axis = r.pair_axis != nullptr ? r.pair_axis[pair] : 0;
-      if (axis < 0 || axis >= r.n_axes) {
-        atomicOr(r.fault, FAULT_BAD_POSITION);
-        axis = 0;
-      }
-      const int32_t p = r.positions != nullptr ? r.positions[(int64_t)axis * r.n_rows + row] : pos;
-      sin_cos((double)p * (double)r.freqs[pair], s[i], c[i]);
     }
+    if (8 * lane < r.rot_dim)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sin_cos(angle(r, 4 * lane + i, at), s[i], c[i]);
   }
 };
 
@@ -214,112 +224,148 @@ __device__ __forceinline__ void turn_head(float (&v)[8], const RopeLaunch &r, bo
   for (int i = 0; i < 8; ++i) v[i] = (float)x[i];
 }
 
-// Heads [h0, h1) of one row, by one wave, 512/D at a time in batches of kBatch
-// loads; the first batch is on its way while the row's cosines are computed.
-// A pair's values, weights, cosine and sine meet in four products that are the
-// row's, so a head costs two products a value and its norm one more.
+// A row's heads [h0, h1) of one kind.
+struct HeadRange {
+  HeadRows m;
+  const void *weight;
+  int h0, h1;
+};
+
+// Heads of one row, by one wave, 512/D at a time in batches of kBatch loads:
+// those of `one`, then those of `two`; the first batch is on its way while the
+// row's cosines are computed, a pair or two a lane, and passed round through
+// `turns` (the wave's own).  A pair's values, weights, cosine and sine meet in
+// four products that are the row's, so a head costs two products a value and
+// its norm one more.
 template <int D, bool kIn16, bool kOut16, bool kAdjacent>
-__device__ __forceinline__ void turn_row(const RopeLaunch &r, const HeadRows &m, const void *weight, int64_t row,
-                                         int32_t pos, int h0, int h1, int lane) {
+__device__ __forceinline__ void turn_row(const RopeLaunch &r, const HeadRange &one, const HeadRange &two, int64_t row,
+                                         int32_t pos, int lane, float2 (&turns)[D / 2]) {
   constexpr int L = D / 8, kHeads = 64 / L, kBatch = 4;
   const int c = lane % L;
   const Dims d(r, c);
-  const bool rotated = 8 * c < r.rot_dim, norm = weight != nullptr;
-  const int64_t src = row * m.stride, dst = row * m.out_stride;
-  float v[kBatch][8];
-  auto load = [&](int first) {
+  const bool rotated = 8 * c < r.rot_dim;
+  float tc[4], ts[4];
+  bool turn = true;
+#pragma unroll 1
+  for (int kind = one.h0 < one.h1 ? 0 : 1; kind < 2; ++kind) {
+    const HeadRange &g = kind == 0 ? one : two;
+    if (g.h0 >= g.h1) break;
+    const bool norm = g.weight != nullptr;
+    const int64_t src = row * g.m.stride, dst = row * g.m.out_stride;
+    float v[kBatch][8];
+    auto load = [&](int first) {
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      if (first + k * kHeads >= h1) break;
-      const int h = min(first + k * kHeads + lane / L, h1 - 1);
-      load4(m.src, src + (int64_t)h * D + d.a, kIn16, v[k], 0);
-      load4(m.src, src + (int64_t)h * D + d.b, kIn16, v[k], 4);
+      for (int k = 0; k < kBatch; ++k) {
+        if (first + k * kHeads >= g.h1) break;
+        const int h = min(first + k * kHeads + lane / L, g.h1 - 1);
+        load4(g.m.src, src + (int64_t)h * D + d.a, kIn16, v[k], 0);
+        load4(g.m.src, src + (int64_t)h * D + d.b, kIn16, v[k], 4);
+      }
+    };
+    load(g.h0);
+    float w[8];
+    load_weight(g.weight, r.norm_bf16 != 0, d, w);
+    if (turn) {
+      int32_t at[4] = {pos, pos, pos, pos};
+      if (r.positions != nullptr)
+#pragma unroll
+        for (int a = 0; a < 4; ++a) at[a] = r.positions[(int64_t)min(a, r.n_axes - 1) * r.n_rows + row];
+#pragma unroll
+      for (int pair = lane; pair < D / 2; pair += 64) {
+        if (2 * pair >= r.rot_dim) break;
+        double s, co;
+        sin_cos(angle(r, pair, at), s, co);
+        turns[pair] = float2{(float)co, (float)s};
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 u = rotated ? turns[4 * c + i] : float2{1.0f, 0.0f};
+        tc[i] = u.x;
+        ts[i] = u.y;
+      }
+      turn = false;
     }
-  };
-  load(h0);
-  float w[8];
-  load_weight(weight, r.norm_bf16 != 0, d, w);
-  // y[a] = x[a] * ca + x[b] * -sb, y[b] = x[b] * cb + x[a] * sa
-  float ca[4], cb[4], sa[4], sb[4];
-  {
-    Turn t;
-    t.load(r, row, pos, c);
+    // y[a] = x[a] * ca + x[b] * -sb, y[b] = x[b] * cb + x[a] * sa
+    float ca[4], cb[4], sa[4], sb[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float wa = w[kAdjacent ? 2 * i : i], wb = w[kAdjacent ? 2 * i + 1 : i + 4];
-      ca[i] = (float)t.c[i] * wa;
-      cb[i] = (float)t.c[i] * wb;
-      sa[i] = (float)t.s[i] * wa;
-      sb[i] = (float)t.s[i] * wb;
+      ca[i] = tc[i] * wa;
+      cb[i] = tc[i] * wb;
+      sa[i] = ts[i] * wa;
+      sb[i] = ts[i] * wb;
     }
-  }
-  for (int first = h0;;) {
+    for (int first = g.h0;;) {
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      if (first + k * kHeads >= h1) break;
-      const int h = first + k * kHeads + lane / L;
-      float f = 1.0f;
-      if (norm) {
-        float q = v[k][0] * v[k][0];
+      for (int k = 0; k < kBatch; ++k) {
+        if (first + k * kHeads >= g.h1) break;
+        const int h = first + k * kHeads + lane / L;
+        float f = 1.0f;
+        if (norm) {
+          float q = v[k][0] * v[k][0];
 #pragma unroll
-        for (int i = 1; i < 8; ++i) q = __builtin_fmaf(v[k][i], v[k][i], q);
-        f = inv_sqrt(lanes_sum<L>(q) * (1.0f / D) + r.eps);
-      }
-      float y[8];
+          for (int i = 1; i < 8; ++i) q = __builtin_fmaf(v[k][i], v[k][i], q);
+          f = inv_sqrt(lanes_sum<L>(q) * (1.0f / D) + r.eps);
+        }
+        float y[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int a = kAdjacent ? 2 * i : i, b = kAdjacent ? 2 * i + 1 : i + 4;
-        y[a] = v[k][a] * ca[i];
-        y[b] = v[k][b] * cb[i];
-        if (rotated) {  // (not a sine of 0: it would make NaN of an infinite partner)
-          y[a] = __builtin_fmaf(v[k][b], -sb[i], y[a]);
-          y[b] = __builtin_fmaf(v[k][a], sa[i], y[b]);
+        for (int i = 0; i < 4; ++i) {
+          const int a = kAdjacent ? 2 * i : i, b = kAdjacent ? 2 * i + 1 : i + 4;
+          y[a] = v[k][a] * ca[i];
+          y[b] = v[k][b] * cb[i];
+          if (rotated) {  // (not a sine of 0: it would make NaN of an infinite partner)
+            y[a] = __builtin_fmaf(v[k][b], -sb[i], y[a]);
+            y[b] = __builtin_fmaf(v[k][a], sa[i], y[b]);
+          }
+        }
+        if (norm) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) y[i] *= f;
+        }
+        if (h < g.h1) {
+          store4(g.m.out, dst + (int64_t)h * D + d.a, kOut16, y, 0);
+          store4(g.m.out, dst + (int64_t)h * D + d.b, kOut16, y, 4);
         }
       }
-      if (norm) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] *= f;
-      }
-      if (h < h1) {
-        store4(m.out, dst + (int64_t)h * D + d.a, kOut16, y, 0);
-        store4(m.out, dst + (int64_t)h * D + d.b, kOut16, y, 4);
-      }
+      first += kBatch * kHeads;
+      if (first >= g.h1) break;
+      load(first);
     }
-    first += kBatch * kHeads;
-    if (first >= h1) break;
-    load(first);
   }
 }
 
 template <int D, bool kIn16, bool kOut16>
-__device__ __forceinline__ void turn_row(const RopeLaunch &r, const HeadRows &m, const void *weight, int64_t row,
-                                         int32_t pos, int h0, int h1, int lane) {
-  if (r.adjacent) turn_row<D, kIn16, kOut16, true>(r, m, weight, row, pos, h0, h1, lane);
-  else turn_row<D, kIn16, kOut16, false>(r, m, weight, row, pos, h0, h1, lane);
+__device__ __forceinline__ void turn_row(const RopeLaunch &r, const HeadRange &one, const HeadRange &two, int64_t row,
+                                         int32_t pos, int lane, float2 (&turns)[D / 2]) {
+  if (r.adjacent) turn_row<D, kIn16, kOut16, true>(r, one, two, row, pos, lane, turns);
+  else turn_row<D, kIn16, kOut16, false>(r, one, two, row, pos, lane, turns);
 }
 #endif  // __HIP_DEVICE_COMPILE__
 
-// Wave x takes head chunk x % (nq + nk) of row x / (nq + nk): nq chunks of
-// `chunk` query heads, then nk of key heads.
+// Four rows a workgroup, a row a wave; blockIdx.y: which `chunk` of the row's
+// query heads and then key heads, counted through.
 template <int D, bool kIn16, bool kOut16>
 __global__ __launch_bounds__(256) void rope_rows_kernel(RopeLaunch r, HeadRows q, HeadRows k, int32_t chunk) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  const int lane = threadIdx.x & 63;
-  const int nq = (q.heads + chunk - 1) / chunk, nk = (k.heads + chunk - 1) / chunk;
-  const int64_t x = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t row = x / (nq + nk);
-  const int at = (int)(x % (nq + nk));
+  __shared__ __attribute__((aligned(16))) float2 turns[4][D / 2];
+  const int wave = (int)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row = (int64_t)blockIdx.x * 4 + wave;
   if (row >= r.n_rows) return;
-  // (one copy of the code: the chunk's rows, heads and weight are the wave's)
-  const bool isq = at < nq;
-  const HeadRows &m = isq ? q : k;
-  const int h0 = (isq ? at : at - nq) * chunk;
-  turn_row<D, kIn16, kOut16>(r, m, isq ? r.q_norm : r.k_norm, row, r.own != nullptr ? r.own[row] : 0, h0,
-                             min(m.heads, h0 + chunk), lane);
+  const int h0 = (int)blockIdx.y * chunk, h1 = h0 + chunk;
+  turn_row<D, kIn16, kOut16>(r, HeadRange{q, r.q_norm, h0, min(h1, q.heads)},
+                             HeadRange{k, r.k_norm, max(h0 - q.heads, 0), min(h1 - q.heads, k.heads)}, row,
+                             r.own != nullptr ? r.own[row] : 0, threadIdx.x & 63, turns[wave]);
 #endif
 }
 
 // ---- append ------------------------------------------------------------------------
+// kv heads of a workgroup, which share a row's cosines: two of a large call's
+// rows (65,619 rows of 2 heads 82.6 -> 62 us), one of a small call's, where
+// the second would wait for the first (64 rows 9.1 -> 12.8 us a call).
+constexpr int append_heads(int rows) { return rows == 32 ? 2 : 1; }
+
 #if defined(__HIP_DEVICE_COMPILE__)
 
 // E2M1 codes of this lane's 8 values of a block held by 4 consecutive lanes,
@@ -358,32 +404,33 @@ __device__ __forceinline__ uint32_t low_nibbles(uint32_t w0, uint32_t w1) {
 #endif  // __HIP_DEVICE_COMPILE__
 
 // Workgroup x of the first append_blocks takes input rows [ROWS*(x / groups),
-// +ROWS) and kv heads [heads*(x % groups), +heads); the others are the query
+// +ROWS) and kv heads [kHeads*(x % groups), +kHeads); the others are the query
 // waves (rope_rows_kernel's, keys none).
 //  1. wave 0 finds each row's page and slot; rows that have none are reported
 //     and skipped.
-//  2. K: 512/D rows a wave, normed and rotated in f64, through LDS into 8
-//     consecutive dims a lane, quantized by 4 lanes a block and stored.
-//  3. V: codes of tokens that are neighbours share words of a page (4 tokens
-//     of a Q8_0 tile's dim, 8 of a 4-bit one's).  A run is the rows that
-//     follow each other inside one such group of slots; the workgroup that
-//     holds its first row takes all of it (rows past its own among them), puts
-//     the codes through LDS and stores whole words.  A run that does not fill
-//     its group leaves the other tokens' bits alone: bytes, and in 4-bit pages
-//     an atomic xor of the words' own bits (another run of the call may hold
-//     the rest of the word).
+//  2. 512/D rows a wave: K normed and rotated in f64, through LDS into 8
+//     consecutive dims a lane, V as it is, both quantized by 4 lanes a block;
+//     codes and scales to LDS.
+//  3. Runs to the pages, a wave each.  A run is the rows that follow each other
+//     inside one group of slots whose V codes share words of a page (4 tokens
+//     of a Q8_0 tile's dim, 8 of a 4-bit one's); the workgroup that holds its
+//     first row takes all of it (rows past its own among them), and stores
+//     whole words, 16 bytes a lane.  A run that does not fill its group leaves
+//     the other tokens' bits alone: bytes, and in 4-bit pages an atomic xor of
+//     the V words' own bits (another run of the call may hold the rest).
 template <int D, bool kMx4, int ROWS, bool kBf16>
-__global__ __launch_bounds__(256) void append_rope_kernel(AppendRopeLaunch p, int32_t groups, int32_t heads,
-                                                          uint32_t append_blocks, int32_t chunk) {
+__global__ __launch_bounds__(256) void append_rope_kernel(AppendRopeLaunch p, int32_t groups, uint32_t append_blocks,
+                                                          int32_t chunk) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  constexpr int L = D / 8, RW = 64 / L, NB = D / 32;
+  constexpr int L = D / 8, RW = 64 / L, NB = D / 32, H = D / 128;
   constexpr int GROUP = kMx4 ? 8 : 4;        // tokens of a V word
-  constexpr int VR = ROWS + GROUP - 1;       // V rows a workgroup may take
+  constexpr int VR = ROWS + GROUP - 1;       // rows a workgroup may take
   constexpr int CB = kMx4 ? D / 2 : D;       // code bytes of a row
-  constexpr int CS = CB + 8;                 // LDS row stride
+  constexpr int CS = CB + 16;                // LDS row stride
+  constexpr int kHeads = append_heads(ROWS);
   __shared__ __attribute__((aligned(16))) float turned[4][RW][D];
-  __shared__ __attribute__((aligned(16))) uint8_t codes[VR][CS];
-  __shared__ uint16_t scales[VR][NB];
+  __shared__ __attribute__((aligned(16))) uint8_t codes[kHeads][2][VR][CS];
+  __shared__ uint16_t scales[kHeads][2][VR][NB];
   __shared__ int64_t rbase[VR + 1];  // the row's page, bytes into the pool; -1: skip
   __shared__ int32_t rslot[VR + 1], rpos[VR + 1];
   __shared__ uint64_t starts;        // rows that start a run
@@ -393,17 +440,17 @@ __global__ __launch_bounds__(256) void append_rope_kernel(AppendRopeLaunch p, in
   const int tid = (int)threadIdx.x, lane = tid & 63;
   const int wave = (int)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (blockIdx.x >= append_blocks) {
-    const int nq = (p.q.heads + chunk - 1) / chunk;
-    const int64_t x = (int64_t)(blockIdx.x - append_blocks) * 4 + wave;
-    const int64_t row = x / nq;
-    const int at = (int)(x % nq);
+    const uint32_t nq = (uint32_t)(p.q.heads + chunk - 1) / (uint32_t)chunk, x = blockIdx.x - append_blocks;
+    const int64_t row = (int64_t)(x / nq) * 4 + wave;
+    const int at = (int)(x % nq) * chunk;
     if (row < a.n_rows)
-      turn_row<D, kBf16, kBf16>(p.r, p.q, p.r.q_norm, row, a.positions[row], at * chunk,
-                                min(p.q.heads, (at + 1) * chunk), lane);
+      turn_row<D, kBf16, kBf16>(p.r, HeadRange{p.q, p.r.q_norm, at, min(p.q.heads, at + chunk)},
+                                HeadRange{p.q, nullptr, 0, 0}, row, a.positions[row], lane,
+                                *reinterpret_cast<float2(*)[D / 2]>(&turned[wave][0][0]));
     return;
   }
   const int64_t row0 = (int64_t)(blockIdx.x / groups) * ROWS;
-  const int h0 = (int)(blockIdx.x % groups) * heads, h1 = min(g.kv_heads, h0 + heads);
+  const int h0 = (int)(blockIdx.x % groups) * kHeads, nh = min(g.kv_heads - h0, kHeads);
   const int nr = (int)min<int64_t>(ROWS, (int64_t)a.n_rows - row0);
   const uint64_t PB = kMx4 ? mx4_page_bytes(g) : page_bytes(g);
   const uint64_t RB = kMx4 ? mx4_region_bytes(g) : region_bytes(g);
@@ -432,7 +479,7 @@ __global__ __launch_bounds__(256) void append_rope_kernel(AppendRopeLaunch p, in
       }
       if (bad != 0 && h0 == 0 && lane < nr) atomicOr(a.fault, bad);
     }
-    const bool follows = (lane > 0 || row0 > 0) && seq == pseq && pos == ppos + 1 && pos % GROUP != 0;
+    const bool follows = (lane > 0 || row0 > 0) && seq == pseq && pos > 0 && pos - 1 == ppos && pos % GROUP != 0;
     const uint64_t s = __ballot(in && !follows);
     if (lane <= VR) {
       rbase[lane] = base;
@@ -447,111 +494,110 @@ __global__ __launch_bounds__(256) void append_rope_kernel(AppendRopeLaunch p, in
     }
   }
   __syncthreads();
+  const uint64_t runs = starts;
+  const int v0 = runs != 0 ? (int)__builtin_ctzll(runs) : 0, v1 = vend;
 
+  // ---- quantized rows to LDS ------------------------------------------------------
   const int c = lane % L, sub = lane / L;
-  // ---- K ----------------------------------------------------------------------
   const Dims d(p.r, c);
   const bool rotated = p.r.on && 8 * c < p.r.rot_dim;
   float w[8];
   load_weight(p.r.on ? p.r.k_norm : nullptr, p.r.norm_bf16 != 0, d, w);
-  for (int i = RW * wave; i < nr; i += 4 * RW) {
-    const int r = min(i + sub, nr - 1);
-    const bool live = i + sub < nr && rbase[r] >= 0;
+  for (int i = v0 + RW * wave; i < v1; i += 4 * RW) {
+    const int r = min(i + sub, v1 - 1);
+    float k[kHeads][8], v[kHeads][8];
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h) {
+      const int64_t hd = (int64_t)(h0 + min(h, nh - 1)) * D;
+      const int64_t ka = (row0 + r) * p.k_stride + hd, va = (row0 + r) * p.v_stride + hd + 8 * c;
+      load4(a.k_src, ka + d.a, kBf16, k[h], 0);
+      load4(a.k_src, ka + d.b, kBf16, k[h], 4);
+      load4(a.v_src, va, kBf16, v[h], 0);
+      load4(a.v_src, va + 4, kBf16, v[h], 4);
+    }
     Turn t;
     if (p.r.on) t.load(p.r, row0 + r, rpos[r], c);
-    for (int h = h0; h < h1; ++h) {
-      float v[8];
-      const int64_t at = (row0 + r) * p.k_stride + (int64_t)h * D;
-      load4(a.k_src, at + d.a, kBf16, v, 0);
-      load4(a.k_src, at + d.b, kBf16, v, 4);
-      if (p.r.on && p.r.adjacent) turn_head<double, D, true>(v, p.r, p.r.k_norm != nullptr, w, t, rotated);
-      else if (p.r.on) turn_head<double, D, false>(v, p.r, p.r.k_norm != nullptr, w, t, rotated);
-      // to 8 consecutive dims a lane, within the wave
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h) {
+      if (h >= nh) break;
+      if (p.r.on && p.r.adjacent) turn_head<double, D, true>(k[h], p.r, p.r.k_norm != nullptr, w, t, rotated);
+      else if (p.r.on) turn_head<double, D, false>(k[h], p.r, p.r.k_norm != nullptr, w, t, rotated);
+      // K to 8 consecutive dims a lane, within the wave
       float *row = turned[wave][sub];
-      *reinterpret_cast<v4f *>(row + d.a) = v4f{v[0], v[1], v[2], v[3]};
-      *reinterpret_cast<v4f *>(row + d.b) = v4f{v[4], v[5], v[6], v[7]};
+      *reinterpret_cast<v4f *>(row + d.a) = v4f{k[h][0], k[h][1], k[h][2], k[h][3]};
+      *reinterpret_cast<v4f *>(row + d.b) = v4f{k[h][4], k[h][5], k[h][6], k[h][7]};
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
       const v4f x0 = *reinterpret_cast<const v4f *>(row + 8 * c), x1 = *reinterpret_cast<const v4f *>(row + 8 * c + 4);
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
       __builtin_amdgcn_wave_barrier();
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        v[k] = x0[k];
-        v[4 + k] = x1[k];
+      for (int e = 0; e < 4; ++e) {
+        k[h][e] = x0[e];
+        k[h][4 + e] = x1[e];
       }
-      const int blk = c / 4;
-      uint8_t *region = a.pages + (live ? rbase[r] : 0) + (uint64_t)(2 * h) * RB;
-      const int slot = rslot[r];
+      uint16_t ks, vs;
       if constexpr (kMx4) {
-        int32_t e;
-        const uint32_t q = mx4_quantize8<0>(v, e);
-        if (live) {
-          uint8_t *tile = region + (uint64_t)(slot / 32) * mx4_tile_bytes(D);
-          const int tok = slot % 32, j = tok % 8 / 4, m = 4 * (tok / 8) + tok % 4, jh = j * (D / 128) + blk / 4;
-          *reinterpret_cast<uint32_t *>(tile + (jh * 4 + blk % 4) * 256 + m * 16 + 4 * (c % 4)) = q;
-          if (c % 4 == 0) tile[16 * D + (blk % 4 * 16 + m) * (D / 64) + jh] = e == 999 ? 255 : (uint8_t)(e + 127);
-        }
+        int32_t ke, ve;
+        const uint32_t kq = mx4_quantize8<0>(k[h], ke), vq = mx4_quantize8<1>(v[h], ve);
+        *reinterpret_cast<uint32_t *>(&codes[h][0][r][4 * c]) = kq;
+        *reinterpret_cast<uint32_t *>(&codes[h][1][r][4 * c]) = vq;
+        ks = ke == 999 ? 255 : (uint16_t)(ke + 127);
+        vs = ve == 999 ? 0x7e : (uint16_t)(4 * (ve + 23));
       } else {
-        uint16_t scale;
-        const uint64_t q = q8_quantize_values<8>(v, a.rule, scale);
-        if (live) {
-          *reinterpret_cast<uint64_t *>(region + (uint64_t)slot * D + 8 * c) = q;
-          if (c % 4 == 0) *reinterpret_cast<uint16_t *>(region + scale_offset(g, slot, blk)) = scale;
-        }
+        const uint64_t kq = q8_quantize_values<8>(k[h], a.rule, ks), vq = q8_quantize_values<8>(v[h], a.rule, vs);
+        *reinterpret_cast<uint64_t *>(&codes[h][0][r][8 * c]) = kq;
+        *reinterpret_cast<uint64_t *>(&codes[h][1][r][8 * c]) = vq ^ 0x8080808080808080ull;  // stored biased (code_bias)
+      }
+      if (c % 4 == 0) {
+        scales[h][0][r][c / 4] = ks;
+        scales[h][1][r][c / 4] = vs;
       }
     }
   }
+  __syncthreads();
 
-  // ---- V ----------------------------------------------------------------------
-  const uint64_t runs = starts;
-  const int v0 = runs != 0 ? (int)__builtin_ctzll(runs) : 0, v1 = vend;
-  for (int h = h0; h < h1; ++h) {
-    if (h > h0) __syncthreads();
-    for (int i = v0 + RW * wave; i < v1; i += 4 * RW) {
-      const int r = min(i + sub, v1 - 1);
-      float v[8];
-      const int64_t at = (row0 + r) * p.v_stride + (int64_t)h * D + 8 * c;
-      load4(a.v_src, at, kBf16, v, 0);
-      load4(a.v_src, at + 4, kBf16, v, 4);
+  // ---- runs to the pages ------------------------------------------------------------
+  int at = 0;
+  for (uint64_t left = runs; left != 0; left &= left - 1, ++at) {
+    const int r = (int)__builtin_ctzll(left);
+    const uint64_t next = left & (left - 1);
+    const int n = (next != 0 ? (int)__builtin_ctzll(next) : v1) - r;  // 1..GROUP rows
+    const int64_t base = rbase[r];
+    if (base < 0) continue;
+    const int slot = rslot[r], first = slot % GROUP;
+    for (int h = 0; h < nh; ++h) {
+      if ((at * nh + h) % 4 != wave) continue;
+      uint8_t *kr = a.pages + base + (uint64_t)(2 * (h0 + h)) * RB, *vr = kr + RB;
+      const auto &kc = codes[h][0], &vc = codes[h][1];
+      const auto &ks = scales[h][0], &vs = scales[h][1];
       if constexpr (kMx4) {
-        int32_t e;
-        const uint32_t q = mx4_quantize8<1>(v, e);
-        *reinterpret_cast<uint32_t *>(&codes[r][4 * c]) = q;
-        if (c % 4 == 0) scales[r][c / 4] = e == 999 ? 0x7e : (uint16_t)(4 * (e + 23));
-      } else {
-        uint16_t scale;
-        const uint64_t q = q8_quantize_values<8>(v, a.rule, scale);
-        *reinterpret_cast<uint64_t *>(&codes[r][8 * c]) = q ^ 0x8080808080808080ull;  // stored biased (code_bias)
-        if (c % 4 == 0) scales[r][c / 4] = scale;
-      }
-    }
-    __syncthreads();
-    // run by run, each by one wave
-    int at = 0;
-    for (uint64_t left = runs; left != 0; left &= left - 1, ++at) {
-      if (at % 4 != wave) continue;
-      const int r = (int)__builtin_ctzll(left);
-      const uint64_t next = left & (left - 1);
-      const int n = (next != 0 ? (int)__builtin_ctzll(next) : v1) - r;  // 1..GROUP rows
-      const int64_t base = rbase[r];
-      if (base < 0) continue;
-      const int slot = rslot[r], first = slot % GROUP;
-      uint8_t *region = a.pages + base + (uint64_t)(2 * h + 1) * RB;
-      if constexpr (kMx4) {
-        uint8_t *tile = region + (uint64_t)(slot / 32) * mx4_tile_bytes(D);
+        const uint64_t tile = (uint64_t)(slot / 32) * mx4_tile_bytes(D);
         const int grp = slot % 32 / 8;
-        if (lane < D / 4) {  // (c, n): 4 words, of the even and odd dims 2n of blocks 2c and 2c + 1
+        if (lane < 32 * H) {  // K: (j, h, b, token of 4), a block each
+          const int jh = lane / 16, b = lane / 4 % 4, m = lane % 4, k = 4 * (jh / H) + m - first;
+          if (k >= 0 && k < n)
+            *reinterpret_cast<v4u *>(kr + tile + (jh * 4 + b) * 256 + (4 * grp + m) * 16) =
+                *reinterpret_cast<const v4u *>(&kc[r + k][16 * (jh % H * 4 + b)]);
+        }
+        if (lane < 32 * H) {  // K scales: (b, token of 4, j, h), bytes that lie side by side
+          const int b = lane / (8 * H), m = lane / (2 * H) % 4, jh = lane % (2 * H), k = 4 * (jh / H) + m - first;
+          if (k >= 0 && k < n)
+            kr[tile + 16 * D + (b * 16 + 4 * grp + m) * 2 * H + jh] = (uint8_t)ks[r + k][jh % H * 4 + b];
+        }
+        if (lane < D / 4) {  // V: (c, n), 4 words, of the even and odd dims 2n of blocks 2c and 2c + 1
           const int cc = lane / 16, nn = lane % 16;
           uint32_t b[2][2] = {{0, 0}, {0, 0}};
-          for (int k = 0; k < n; ++k) {
-            const int t = first + k;
 #pragma unroll
-            for (int u = 0; u < 2; ++u) b[u][t / 4] |= (uint32_t)codes[r + k][32 * cc + 16 * u + nn] << (8 * (t % 4));
+          for (int t = 0; t < 8; ++t) {
+            if (t < first || t >= first + n) continue;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+              b[u][t / 4] |= (uint32_t)vc[r + t - first][32 * cc + 16 * u + nn] << (8 * (t % 4));
           }
-          v4u q = {low_nibbles(b[0][0], b[0][1]), low_nibbles(b[0][0] >> 4, b[0][1] >> 4),
-                   low_nibbles(b[1][0], b[1][1]), low_nibbles(b[1][0] >> 4, b[1][1] >> 4)};
-          uint32_t *dst = reinterpret_cast<uint32_t *>(tile + cc * 1024 + (grp * 16 + nn) * 16);
+          const v4u q = {low_nibbles(b[0][0], b[0][1]), low_nibbles(b[0][0] >> 4, b[0][1] >> 4),
+                         low_nibbles(b[1][0], b[1][1]), low_nibbles(b[1][0] >> 4, b[1][1] >> 4)};
+          uint32_t *dst = reinterpret_cast<uint32_t *>(vr + tile + cc * 1024 + (grp * 16 + nn) * 16);
           if (n == 8) {
             *reinterpret_cast<v4u *>(dst) = q;
           } else {
@@ -566,22 +612,28 @@ __global__ __launch_bounds__(256) void append_rope_kernel(AppendRopeLaunch p, in
         }
         if (lane < NB * 8) {
           const int blk = lane / 8, k = lane % 8 - first;
-          if (k >= 0 && k < n) tile[16 * D + (grp * NB + blk) * 8 + lane % 8] = (uint8_t)scales[r + k][blk];
+          if (k >= 0 && k < n) vr[tile + 16 * D + (grp * NB + blk) * 8 + lane % 8] = (uint8_t)vs[r + k][blk];
         }
       } else {
+        // K rows of neighbouring slots lie one behind the other
+        if (16 * lane < n * D) {
+          const int k = 16 * lane / D, x = 16 * lane % D;
+          *reinterpret_cast<v4u *>(kr + (uint64_t)slot * D + 16 * lane) = *reinterpret_cast<const v4u *>(&kc[r + k][x]);
+        }
         for (int x = lane; x < D; x += 64) {
-          uint8_t *dst = region + code_offset(g, 1, slot, x);
+          uint8_t *dst = vr + code_offset(g, 1, slot, x);
           if (n == 4) {
-            *reinterpret_cast<uint32_t *>(dst) = (uint32_t)codes[r][x] | (uint32_t)codes[r + 1][x] << 8 |
-                                                 (uint32_t)codes[r + 2][x] << 16 | (uint32_t)codes[r + 3][x] << 24;
+            *reinterpret_cast<uint32_t *>(dst) = (uint32_t)vc[r][x] | (uint32_t)vc[r + 1][x] << 8 |
+                                                 (uint32_t)vc[r + 2][x] << 16 | (uint32_t)vc[r + 3][x] << 24;
           } else {
-            for (int k = 0; k < n; ++k) dst[k] = codes[r + k][x];
+            for (int k = 0; k < n; ++k) dst[k] = vc[r + k][x];
           }
         }
-        if (lane < NB * 4) {
-          const int blk = lane / 4, k = lane % 4;
+        if (lane < NB * 8) {
+          const int kind = lane / (NB * 4), blk = lane / 4 % NB, k = lane % 4;
           if (k < n)
-            *reinterpret_cast<uint16_t *>(region + scale_offset(g, slot + k, blk)) = scales[r + k][blk];
+            *reinterpret_cast<uint16_t *>((kind ? vr : kr) + scale_offset(g, slot + k, blk)) =
+                kind ? vs[r + k][blk] : ks[r + k][blk];
         }
       }
     }
@@ -591,76 +643,78 @@ __global__ __launch_bounds__(256) void append_rope_kernel(AppendRopeLaunch p, in
 
 // ---- rows read back -----------------------------------------------------------------
 
-// One thread per 8 consecutive dims of (row, kv head, kind).
+// One thread per 8 consecutive dims of a row; blockIdx.y: (kv head, kind).
 template <int D, bool kMx4>
 __global__ __launch_bounds__(256) void read_rows_kernel(ReadRowsLaunch p) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  constexpr int L = D / 8;
+  constexpr int L = D / 8, NB = D / 32;
   const AppendLaunch &a = p.a;
   const Geo g = a.g;
-  const int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int c = (int)(x % L);
-  const int kind = (int)(x / L % 2);
-  const int h = (int)(x / (2 * L) % g.kv_heads);
-  const int64_t row = x / (2 * L) / g.kv_heads;
+  const int c = (int)threadIdx.x % L;
+  const int kind = (int)blockIdx.y & 1, h = (int)blockIdx.y >> 1;
+  const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+  void *out = kind == 0 ? p.k_out : p.v_out;
   if (row >= a.n_rows) return;
   const int32_t seq = a.seq_ids[row], pos = a.positions[row];
   int32_t bad = 0, page = 0;
+  const uint32_t upos = (uint32_t)pos, PT = (uint32_t)g.page_tokens;
   if (seq < 0 || seq >= a.n_seqs) bad = FAULT_BAD_SEQ;
-  else if (pos < 0 || pos / g.page_tokens >= a.bt_stride) bad = FAULT_BAD_POSITION;
+  else if (pos < 0 || upos / PT >= (uint32_t)a.bt_stride) bad = FAULT_BAD_POSITION;
   else {
-    page = a.bt[(int64_t)seq * a.bt_stride + pos / g.page_tokens];
+    page = a.bt[(int64_t)seq * a.bt_stride + upos / PT];
     if (page < 0 || page >= g.num_pages) bad = FAULT_BAD_PAGE;
   }
-  if (bad != 0 && c == 0 && kind == 0 && h == 0) atomicOr(a.fault, bad);
-  float v[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-  if (bad == 0) {
-    const int slot = pos % g.page_tokens, blk = c / 4;
-    if constexpr (kMx4) {
-      const uint8_t *tile =
-          a.pages + mx4_region_base(g, page, h, kind) + (uint64_t)(slot / 32) * mx4_tile_bytes(D);
+  if (bad != 0 && c == 0 && blockIdx.y == 0) atomicOr(a.fault, bad);
+  if (out == nullptr) return;
+  const int64_t at = (row * g.kv_heads + h) * D + 8 * c;
+  const int slot = (int)(upos % PT), blk = c / 4;
+  if constexpr (kMx4) {
+    uint32_t q = 0, s = 0;
+    if (bad == 0) {
+      const uint8_t *tile = a.pages + mx4_region_base(g, page, h, kind) + (uint64_t)(slot / 32) * mx4_tile_bytes(D);
       const int tok = slot % 32;
-      float scale;
-      uint32_t q;
       if (kind == 0) {
         const int j = tok % 8 / 4, m = 4 * (tok / 8) + tok % 4, jh = j * (D / 128) + blk / 4;
         q = *reinterpret_cast<const uint32_t *>(tile + (jh * 4 + blk % 4) * 256 + m * 16 + 4 * (c % 4));
-        const uint32_t s = tile[16 * D + (blk % 4 * 16 + m) * (D / 64) + jh];
-        scale = s == 255 ? __builtin_nanf("") : __builtin_bit_cast(float, s << 23);
+        s = tile[16 * D + (blk % 4 * 16 + m) * (D / 64) + jh];
       } else {
         const int grp = tok / 8, nib = 4 * (tok % 8);
-        q = 0;
+        v2u w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {  // dims 32*blk + 8*(c % 4) + 2*i, +1
-          const v2u w = *reinterpret_cast<const v2u *>(tile + blk / 2 * 1024 + (grp * 16 + 4 * (c % 4) + i) * 16 +
-                                                       8 * (blk % 2));
-          q |= (w[0] >> nib & 15u) << (8 * i) | (w[1] >> nib & 15u) << (8 * i + 4);
-        }
-        const uint32_t s = tile[16 * D + (grp * (D / 32) + blk) * 8 + tok % 8];
-        scale = s >= 0x7c ? __builtin_nanf("") : __builtin_bit_cast(float, (s / 4 - 23 + 127) << 23);
-      }
+        for (int i = 0; i < 4; ++i)  // dims 32*blk + 8*(c % 4) + 2*i, +1
+          w[i] = *reinterpret_cast<const v2u *>(tile + blk / 2 * 1024 + (grp * 16 + 4 * (c % 4) + i) * 16 + 8 * (blk % 2));
+        s = tile[16 * D + (grp * NB + blk) * 8 + tok % 8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        // 0, 0.5, 1, 1.5, 2, 3, 4, 6: the code as an f32 with one mantissa bit, 0 and 0.5 apart
-        const uint32_t n = q >> (4 * i) & 15u, u = n & 7u;
-        const float m = u < 2 ? 0.5f * (float)u : __builtin_bit_cast(float, (u / 2 + 126u) << 23 | (u & 1u) << 22);
-        v[i] = (n & 8u ? -m : m) * scale;
+        for (int i = 0; i < 4; ++i) q |= (w[i][0] >> nib & 15u) << (8 * i) | (w[i][1] >> nib & 15u) << (8 * i + 4);
+        s = s >= 0x7c ? 255 : s / 4 - 23 + 127;  // as K's
       }
+    }
+    const float scale = __builtin_bit_cast(float, s << 23);  // (255: NaN)
+    if (p.out_bf16 != 0) {
+      const v2b w0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, scale, 0), w1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, scale, 1),
+                w2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, scale, 2), w3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, scale, 3);
+      *reinterpret_cast<v4u *>(static_cast<uint16_t *>(out) + at) =
+          v4u{__builtin_bit_cast(uint32_t, w0), __builtin_bit_cast(uint32_t, w1), __builtin_bit_cast(uint32_t, w2),
+              __builtin_bit_cast(uint32_t, w3)};
     } else {
+      const v2f w0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, scale, 0), w1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, scale, 1),
+                w2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, scale, 2), w3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, scale, 3);
+      v4f *dst = reinterpret_cast<v4f *>(static_cast<float *>(out) + at);
+      dst[0] = v4f{w0[0], w0[1], w1[0], w1[1]};
+      dst[1] = v4f{w2[0], w2[1], w3[0], w3[1]};
+    }
+  } else {
+    float v[8] = {};
+    if (bad == 0) {
       const uint8_t *region = a.pages + region_base(g, page, h, kind);
       const float scale = f16_bits_to_f32(*reinterpret_cast<const uint16_t *>(region + scale_offset(g, slot, blk)));
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         v[i] = scale * (float)(int8_t)(region[code_offset(g, kind, slot, 8 * c + i)] ^ code_bias(kind));
     }
+    store4(out, at, p.out_bf16 != 0, v, 0);
+    store4(out, at + 4, p.out_bf16 != 0, v, 4);
   }
-  void *out = kind == 0 ? p.k_out : p.v_out;
-  if (out == nullptr) return;
-  const int64_t at = (row * g.kv_heads + h) * D + 8 * c;
-  store4(out, at, p.out_bf16 != 0, v, 0);
-  store4(out, at + 4, p.out_bf16 != 0, v, 4);
 #endif  // __HIP_DEVICE_COMPILE__
 }
 
@@ -674,24 +728,20 @@ int32_t head_chunk(int64_t rows, int32_t heads, int32_t per) {
 template <int D, bool kMx4, int ROWS>
 void launch_append_rope_r(const AppendRopeLaunch &p, hipStream_t s) {
   const int64_t row_blocks = ((int64_t)p.a.n_rows + ROWS - 1) / ROWS;
-  // every head of the rows in one workgroup (their cosines are the same) where that leaves 2 a CU
-  const int32_t H = p.a.g.kv_heads;
-  int32_t heads = H;
-  while (heads > 1 && row_blocks * ((H + heads - 1) / heads) < 2 * kComputeUnits) heads = (heads + 1) / 2;
-  const int32_t groups = (H + heads - 1) / heads;
+  const int32_t groups = (p.a.g.kv_heads + append_heads(ROWS) - 1) / append_heads(ROWS);
   const uint32_t blocks = (uint32_t)(row_blocks * groups);
   uint32_t q_blocks = 0;
   int32_t chunk = 1;
   if (ROWS == 8 && p.q.src != nullptr && p.q.bf16 == p.q.out_bf16) {
     chunk = head_chunk(p.a.n_rows, p.q.heads, 512 / D);
-    q_blocks = (uint32_t)(((int64_t)p.a.n_rows * ((p.q.heads + chunk - 1) / chunk) + 3) / 4);
+    q_blocks = (uint32_t)((p.a.n_rows + 3LL) / 4 * ((p.q.heads + chunk - 1) / chunk));
   }
   if (p.a.src_bf16)
     hipLaunchKernelGGL((append_rope_kernel<D, kMx4, ROWS, true>), dim3(blocks + q_blocks), dim3(256), 0, s, p, groups,
-                       heads, blocks, chunk);
+                       blocks, chunk);
   else
     hipLaunchKernelGGL((append_rope_kernel<D, kMx4, ROWS, false>), dim3(blocks + q_blocks), dim3(256), 0, s, p, groups,
-                       heads, blocks, chunk);
+                       blocks, chunk);
 }
 // 32-row workgroups once there are at least 8 per CU, else 8-row ones, which
 // take the queries into the launch: a large call's go by themselves, since the
@@ -713,8 +763,7 @@ hipError_t launch_rope_rows(const RopeLaunch &r, const HeadRows &q, const HeadRo
                             hipStream_t s) {
   if (r.n_rows <= 0 || q.heads + k.heads <= 0) return hipSuccess;
   const int32_t chunk = head_chunk(r.n_rows, q.heads + k.heads, 512 / head_dim);
-  const int64_t waves = (int64_t)r.n_rows * ((q.heads + chunk - 1) / chunk + (k.heads + chunk - 1) / chunk);
-  const dim3 grid((unsigned)((waves + 3) / 4));
+  const dim3 grid((unsigned)((r.n_rows + 3LL) / 4), (unsigned)((q.heads + k.heads + chunk - 1) / chunk));
   const HeadRows &m = q.heads > 0 ? q : k;
   auto go = [&](auto d) {
     constexpr int D = decltype(d)::value;
@@ -746,8 +795,8 @@ hipError_t launch_append_rope(const AppendRopeLaunch &p, hipStream_t s) {
 
 hipError_t launch_read_rows(const ReadRowsLaunch &p, hipStream_t s) {
   if (p.a.n_rows <= 0) return hipSuccess;
-  const int64_t threads = (int64_t)p.a.n_rows * p.a.g.kv_heads * 2 * (p.a.g.head_dim / 8);
-  const dim3 grid((unsigned)((threads + 255) / 256));
+  const int rows = 256 / (p.a.g.head_dim / 8);  // of a workgroup
+  const dim3 grid((unsigned)(((int64_t)p.a.n_rows + rows - 1) / rows), (unsigned)p.a.g.kv_heads * 2);
   if (p.a.g.head_dim == 256) {
     if (p.mx4) hipLaunchKernelGGL((read_rows_kernel<256, true>), grid, dim3(256), 0, s, p);
     else hipLaunchKernelGGL((read_rows_kernel<256, false>), grid, dim3(256), 0, s, p);

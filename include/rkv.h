@@ -344,13 +344,18 @@ size_t rkv_prefill_workspace_bytes(const rkv_kv_geometry *g, const rkv_prefill_a
  * bytes a block.  e is the smallest exponent with max|v| <= 7 * 2^e, kept
  * within -24..15 for K and -22..7 for V; a code is v / 2^e rounded to nearest,
  * ties to the even code, saturating at 6.  A block with a value that is not
- * finite reads back as NaN.  Pages have the geometry, allocator, block tables
- * and copy-on-write copies of the Q8_0 ones, with page_tokens 32, 64, 128 or
- * 256 and rkv_mx4_page_bytes bytes; their layout is internal (rkv_append_rope
- * writes and rkv_read_rows reads them).  No counterpart in the reference,
+ * finite reads back as NaN.  Pages have the geometry, allocator and block tables
+ * of the Q8_0 ones, with page_tokens 32, 64, 128 or 256 and rkv_mx4_page_bytes
+ * bytes, in device memory; their layout is internal (rkv_append_rope writes
+ * and rkv_read_rows reads them).  A pool holds them with
+ * rkv_pool_create_format.  No counterpart in the reference,
  * whose flash decode reads Q8_0 only (har/shaders/flash_decode_q8.comp:1-25);
  * har/crates/r4kv's own 4-bit format packs integer codes under an f16 scale. */
 size_t rkv_mx4_page_bytes(const rkv_kv_geometry *g);
+/* rkv_copy_pages of 4-bit pages. */
+rkv_status rkv_mx4_copy_pages(rkv_ctx *ctx, const rkv_kv_geometry *g, void *pages,
+                              int64_t layer_stride_bytes, int32_t layers,
+                              const int32_t *pairs, int32_t n_pairs, void *stream);
 
 /* rkv_decode_q8 over 4-bit pages: the same arguments, workspace rules and
  * faults, but args->append must be NULL (RKV_ERR_UNSUPPORTED; append with
@@ -547,6 +552,14 @@ typedef struct rkv_pool_desc {
 } rkv_pool_desc;
 typedef struct rkv_pool rkv_pool;
 rkv_status rkv_pool_create(rkv_ctx *ctx, const rkv_pool_desc *desc, rkv_pool **out);
+/* A pool of pages of format RKV_CACHE_Q8 (rkv_pool_create) or RKV_CACHE_MX4.
+ * Over 4-bit pages rkv_pool_decode and rkv_pool_prefill are rkv_decode_mx4 and
+ * rkv_prefill_mx4, with their workspaces, and rows come and go by
+ * rkv_pool_append_rope and rkv_pool_read_rows; RKV_ERR_UNSUPPORTED there:
+ * RKV_PAGES_HOST, and the calls that carry Q8_0 rows (rkv_pool_append,
+ * _gather, _spill, _restore). */
+rkv_status rkv_pool_create_format(rkv_ctx *ctx, const rkv_pool_desc *desc, int32_t format,
+                                  rkv_pool **out);
 rkv_status rkv_pool_destroy(rkv_pool *pool);
 /* The pool forgets `stream` if its previous call was queued there: the work
  * queued on it so far is marked (an event recorded now), and the next call,
@@ -573,6 +586,13 @@ const int32_t *rkv_pool_block_tables(rkv_pool *pool); /* [max_seqs][max_pages_pe
 const int32_t *rkv_pool_seq_lens(rkv_pool *pool);     /* [max_seqs] */
 rkv_status rkv_pool_append(rkv_pool *pool, int32_t layer, const rkv_append_args *args,
                            void *stream);
+/* rkv_append_rope on a layer; args->format is the pool's. */
+rkv_status rkv_pool_append_rope(rkv_pool *pool, int32_t layer, const rkv_append_rope_args *args,
+                                void *stream);
+/* rkv_read_rows on a layer. */
+rkv_status rkv_pool_read_rows(rkv_pool *pool, int32_t layer, int32_t n_rows, const int32_t *seq_ids,
+                              const int32_t *positions, void *k_out, void *v_out, int32_t out_dtype,
+                              void *stream);
 rkv_status rkv_pool_decode(rkv_pool *pool, int32_t layer, const rkv_decode_args *args,
                            void *stream);
 /* rkv_prefill_q8 on a layer; also checks ctx_lens[e] + q_rows[e] against the

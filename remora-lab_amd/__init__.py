@@ -181,6 +181,8 @@ _SIGS = {
     "rkv_alloc_take_copies": (C.c_int32, [P, P, C.c_int32, I32P]),
     "rkv_copy_pages": (C.c_int32, [P, C.POINTER(Geometry), P, C.c_int64, C.c_int32, P,
                                    C.c_int32, P]),
+    "rkv_mx4_copy_pages": (C.c_int32, [P, C.POINTER(Geometry), P, C.c_int64, C.c_int32, P,
+                                       C.c_int32, P]),
     "rkv_append_q8": (C.c_int32, [P, C.POINTER(Geometry), P, P, C.c_int32, C.c_int32,
                                   C.POINTER(AppendArgs), P]),
     "rkv_decode_q8": (C.c_int32, [P, C.POINTER(Geometry), P, P, C.c_int32, P, C.c_int32,
@@ -210,6 +212,9 @@ _SIGS = {
     "rkv_flash_decode_scratch_bytes": (C.c_size_t, [C.POINTER(FlashDecodeParams)]),
     "rkv_flash_decode_q8": (C.c_int32, [P, C.POINTER(FlashDecodeParams), P, P, P, P, P, P]),
     "rkv_pool_create": (C.c_int32, [P, C.POINTER(PoolDesc), C.POINTER(P)]),
+    "rkv_pool_create_format": (C.c_int32, [P, C.POINTER(PoolDesc), C.c_int32, C.POINTER(P)]),
+    "rkv_pool_append_rope": (C.c_int32, [P, C.c_int32, C.POINTER(AppendRopeArgs), P]),
+    "rkv_pool_read_rows": (C.c_int32, [P, C.c_int32, C.c_int32, P, P, P, P, C.c_int32, P]),
     "rkv_pool_destroy": (C.c_int32, [P]),
     "rkv_pool_release_stream": (C.c_int32, [P, P]),
     "rkv_pool_allocator": (P, [P]),
@@ -778,6 +783,12 @@ def _append_args(ctx, g, fmt, seq_ids, positions, k_src, v_src, rope, q, q_out, 
 def read_rows(ctx: Ctx, g: Geometry, fmt: int, pages, block_tables, seq_ids, positions, k_out, v_out,
               stream=None) -> None:
     """Values of cached rows into k_out, v_out [n][kv_heads][head_dim] (either may be None)."""
+    rows = _read_args(ctx, g, seq_ids, positions, k_out, v_out)
+    check(lib().rkv_read_rows(ctx.h, C.byref(g), fmt, pages.data_ptr(), _i32(block_tables, "block_tables"),
+                              block_tables.shape[-1], block_tables.shape[0], *rows, _raw_stream(ctx, stream)))
+
+
+def _read_args(ctx, g, seq_ids, positions, k_out, v_out) -> tuple:
     n, kv, D, dev = seq_ids.numel(), g.kv_heads, g.head_dim, ctx.device
     out = k_out if k_out is not None else v_out
     if positions.numel() != n:
@@ -791,10 +802,15 @@ def read_rows(ctx: Ctx, g: Geometry, fmt: int, pages, block_tables, seq_ids, pos
         if h != kv or s != kv * D:
             raise ValueError("outputs: contiguous [rows][kv_heads][head_dim]")
         at.append(p)
-    check(lib().rkv_read_rows(ctx.h, C.byref(g), fmt, pages.data_ptr(), _i32(block_tables, "block_tables"),
-                              block_tables.shape[-1], block_tables.shape[0], n, _i32(seq_ids, "seq_ids"),
-                              _i32(positions, "positions"), *at,
-                              _type(out.dtype) if out is not None else F32, _raw_stream(ctx, stream)))
+    return (n, _i32(seq_ids, "seq_ids"), _i32(positions, "positions"), *at,
+            _type(out.dtype) if out is not None else F32)
+
+
+def mx4_copy_pages(ctx: Ctx, g: Geometry, pages, layer_stride: int, layers: int, pairs,
+                   n_pairs: int, stream=None) -> None:
+    """copy_pages of 4-bit pages."""
+    check(lib().rkv_mx4_copy_pages(ctx.h, C.byref(g), _ptr(pages), layer_stride, layers,
+                                   _ptr(pairs), n_pairs, _raw_stream(ctx, stream)))
 
 
 def mx4_page_bytes(g: Geometry) -> int:
@@ -867,13 +883,14 @@ class Pool:
     """Device pages for `layers` layers + allocator + device block tables."""
 
     def __init__(self, ctx: Ctx, layers, kv_heads, head_dim, page_tokens, num_pages, max_seqs,
-                 max_pages_per_seq, seed=0, page_memory=0):
+                 max_pages_per_seq, seed=0, page_memory=0, page_format=CACHE_Q8):
         self.ctx = ctx
         d = PoolDesc(layers, kv_heads, head_dim, page_tokens, num_pages, max_seqs,
                      max_pages_per_seq, seed, page_memory)
         h = P()
-        check(lib().rkv_pool_create(ctx.h, C.byref(d), C.byref(h)))
+        check(lib().rkv_pool_create_format(ctx.h, C.byref(d), page_format, C.byref(h)))
         self.h = h
+        self.page_format = page_format
         self.desc = d
         self.geometry = Geometry(kv_heads, head_dim, page_tokens, num_pages)
         self.alloc = Allocator(num_pages, page_tokens, max_seqs, max_pages_per_seq,
@@ -902,6 +919,18 @@ class Pool:
         a = AppendArgs(seq_ids.numel(), _ptr(seq_ids), _ptr(positions), _ptr(k_src),
                        _ptr(v_src), dtype, rule)
         check(lib().rkv_pool_append(self.h, layer, C.byref(a), _stream(stream)))
+
+    def append_rope(self, layer, seq_ids, positions, k_src, v_src, rope: RopeArgs | None = None, q=None,
+                    q_out=None, rule=Q8_CANONICAL, stream=None) -> None:
+        """append_rope on a layer, in the pool's page format."""
+        a = _append_args(self.ctx, self.geometry, self.page_format, seq_ids, positions, k_src, v_src, rope, q,
+                         q_out, rule)
+        check(lib().rkv_pool_append_rope(self.h, layer, C.byref(a), _raw_stream(self.ctx, stream)))
+
+    def read_rows(self, layer, seq_ids, positions, k_out, v_out, stream=None) -> None:
+        """read_rows on a layer."""
+        rows = _read_args(self.ctx, self.geometry, seq_ids, positions, k_out, v_out)
+        check(lib().rkv_pool_read_rows(self.h, layer, *rows, _raw_stream(self.ctx, stream)))
 
     def decode(self, layer, a: DecodeArgs, stream=None) -> None:
         check(lib().rkv_pool_decode(self.h, layer, C.byref(a), _stream(stream)))

@@ -1245,6 +1245,9 @@ rkv_status check_format(const rkv_kv_geometry *g, int32_t format, const char *op
   if (format == RKV_CACHE_MX4) return check_mx4_geometry(g, op);
   return fail(RKV_ERR_UNSUPPORTED, op, "format=%d", format);
 }
+int64_t format_page_bytes(const rkv_kv_geometry *g, int32_t format) {
+  return format == RKV_CACHE_MX4 ? (int64_t)rkv_mx4_page_bytes(g) : (int64_t)rkv::page_bytes(to_geo(g));
+}
 }  // namespace
 
 extern "C" {
@@ -1472,7 +1475,7 @@ rkv_status rkv_decode_mx4(rkv_ctx *ctx, const rkv_kv_geometry *g, const void *pa
   if (rkv_status s = check_tables(pages, block_tables, bt_stride, n_seqs, op)) return s;
   if (!seq_lens) return fail(RKV_ERR_INVALID_ARG, op, "seq_lens is NULL");
   if (a->append)
-    return fail(RKV_ERR_UNSUPPORTED, op, "append: 4-bit rows are appended by rkv_append_mx4 or rkv_append_rope");
+    return fail(RKV_ERR_UNSUPPORTED, op, "append: 4-bit rows are appended by rkv_append_rope");
   if (rkv_status s = use_device(ctx, op)) return s;
   if (a->batch == 0) return RKV_OK;
   return run_decode(ctx, g, pages, block_tables, bt_stride, seq_lens, n_seqs, a, stream, mx4_plan_of(g, a),
@@ -1554,13 +1557,13 @@ rkv_status rkv_import_q8(rkv_ctx *ctx, const rkv_kv_geometry *g, void *pages,
   return e == hipSuccess ? RKV_OK : hip_fail(op, e);
 }
 
-rkv_status rkv_copy_pages(rkv_ctx *ctx, const rkv_kv_geometry *g, void *pages,
-                          int64_t layer_stride_bytes, int32_t layers, const int32_t *pairs,
-                          int32_t n_pairs, void *stream) {
-  const char *op = "rkv_copy_pages";
+namespace {
+rkv_status copy_pages(rkv_ctx *ctx, const rkv_kv_geometry *g, int32_t format, void *pages,
+                      int64_t layer_stride_bytes, int32_t layers, const int32_t *pairs,
+                      int32_t n_pairs, void *stream, const char *op) {
   if (rkv_status s = use_device(ctx, op)) return s;
-  if (rkv_status s = check_geometry(g, op)) return s;
-  const int64_t pb = (int64_t)rkv::page_bytes(to_geo(g));
+  if (rkv_status s = check_format(g, format, op)) return s;
+  const int64_t pb = format_page_bytes(g, format);
   if (layers < 1 || n_pairs < 0)
     return fail(RKV_ERR_INVALID_ARG, op, "layers=%d n_pairs=%d", layers, n_pairs);
   if (layers > 1 && layer_stride_bytes < pb * g->num_pages)
@@ -1571,6 +1574,21 @@ rkv_status rkv_copy_pages(rkv_ctx *ctx, const rkv_kv_geometry *g, void *pages,
   hipError_t e = rkv::launch_copy_pages(static_cast<uint8_t *>(pages), layer_stride_bytes, layers,
                                         g->num_pages, pairs, n_pairs, pb, as_stream(stream));
   return e == hipSuccess ? RKV_OK : hip_fail(op, e);
+}
+}  // namespace
+
+rkv_status rkv_copy_pages(rkv_ctx *ctx, const rkv_kv_geometry *g, void *pages,
+                          int64_t layer_stride_bytes, int32_t layers, const int32_t *pairs,
+                          int32_t n_pairs, void *stream) {
+  return copy_pages(ctx, g, RKV_CACHE_Q8, pages, layer_stride_bytes, layers, pairs, n_pairs, stream,
+                    "rkv_copy_pages");
+}
+
+rkv_status rkv_mx4_copy_pages(rkv_ctx *ctx, const rkv_kv_geometry *g, void *pages,
+                              int64_t layer_stride_bytes, int32_t layers, const int32_t *pairs,
+                              int32_t n_pairs, void *stream) {
+  return copy_pages(ctx, g, RKV_CACHE_MX4, pages, layer_stride_bytes, layers, pairs, n_pairs, stream,
+                    "rkv_mx4_copy_pages");
 }
 
 rkv_status rkv_f32_to_f16(rkv_ctx *ctx, const float *in, uint16_t *out, int64_t n, int32_t rule,
@@ -1679,6 +1697,7 @@ struct rkv_pool {
   rkv_ctx *ctx = nullptr;
   rkv_pool_desc d{};
   rkv_kv_geometry g{};
+  int32_t format = RKV_CACHE_Q8;
   rkv_alloc *alloc = nullptr;
   uint8_t *pages = nullptr;  // layers * num_pages * page_bytes (device address)
   void *host_pages = nullptr;  // RKV_PAGES_HOST: the pinned allocation behind `pages`
@@ -1718,6 +1737,10 @@ struct rkv_pool {
 };
 
 namespace {
+// calls whose rows are Q8_0 blocks
+rkv_status check_q8_pool(const rkv_pool *p, const char *op) {
+  return p->format == RKV_CACHE_Q8 ? RKV_OK : fail(RKV_ERR_UNSUPPORTED, op, "the pool holds 4-bit pages");
+}
 size_t stage_ints(const rkv_pool_desc &d) {
   return (size_t)d.max_seqs * (d.max_pages_per_seq + 1) + d.max_seqs + 2 * (size_t)d.num_pages;
 }
@@ -1783,6 +1806,10 @@ rkv_status order_after_last(rkv_pool *p, hipStream_t hs, const char *op) {
 extern "C" {
 
 rkv_status rkv_pool_create(rkv_ctx *ctx, const rkv_pool_desc *desc, rkv_pool **out) {
+  return rkv_pool_create_format(ctx, desc, RKV_CACHE_Q8, out);
+}
+
+rkv_status rkv_pool_create_format(rkv_ctx *ctx, const rkv_pool_desc *desc, int32_t format, rkv_pool **out) {
   const char *op = "rkv_pool_create";
   if (rkv_status s = use_device(ctx, op)) return s;
   if (!desc || !out) return fail(RKV_ERR_INVALID_ARG, op, "NULL argument");
@@ -1791,18 +1818,23 @@ rkv_status rkv_pool_create(rkv_ctx *ctx, const rkv_pool_desc *desc, rkv_pool **o
   if (desc->page_memory != RKV_PAGES_DEVICE && desc->page_memory != RKV_PAGES_HOST)
     return fail(RKV_ERR_INVALID_ARG, op, "page_memory=%d", desc->page_memory);
   rkv_kv_geometry g{desc->kv_heads, desc->head_dim, desc->page_tokens, desc->num_pages};
-  if (rkv_status s = check_geometry(&g, op)) return s;
+  if (rkv_status s = check_format(&g, format, op)) return s;
+  // a run of rows that ends inside a group of 8 tokens changes its nibbles by
+  // atomics, which the host link does not carry
+  if (format == RKV_CACHE_MX4 && desc->page_memory == RKV_PAGES_HOST)
+    return fail(RKV_ERR_UNSUPPORTED, op, "page_memory=%d (4-bit pages: RKV_PAGES_DEVICE)", desc->page_memory);
   rkv_alloc_desc ad{desc->num_pages, desc->page_tokens, desc->max_seqs, desc->max_pages_per_seq,
                     desc->free_list_seed};
   rkv_pool *p = new rkv_pool;
   p->ctx = ctx;
   p->d = *desc;
   p->g = g;
+  p->format = format;
   if (rkv_status s = rkv_alloc_create(&ad, &p->alloc)) {
     delete p;
     return s;
   }
-  p->layer_bytes = (size_t)desc->num_pages * rkv::page_bytes(to_geo(&g));
+  p->layer_bytes = (size_t)desc->num_pages * format_page_bytes(&g, format);
   hipError_t e;
   const size_t tbytes = sizeof(int32_t) * (size_t)desc->max_seqs * desc->max_pages_per_seq;
   const size_t sbytes = sizeof(int32_t) * stage_ints(*desc);
@@ -1956,7 +1988,7 @@ rkv_status rkv_pool_sync_tables(rkv_pool *p, void *stream) {
   ++p->n_syncs;
   if ((e = rkv::launch_copy_pages(p->pages, (int64_t)p->layer_bytes, p->d.layers, p->d.num_pages,
                                   d + pairs_at, n_pairs,
-                                  (int64_t)rkv::page_bytes(to_geo(&p->g)), hs)) != hipSuccess)
+                                  format_page_bytes(&p->g, p->format), hs)) != hipSuccess)
     return hip_fail(op, e);
   const unsigned long long blocks = (unsigned long long)n_rows + 1;
   const unsigned long long seq = p->n_syncs;
@@ -1979,11 +2011,37 @@ const int32_t *rkv_pool_seq_lens(rkv_pool *p) { return p ? p->d_lens : nullptr; 
 rkv_status rkv_pool_append(rkv_pool *p, int32_t layer, const rkv_append_args *args, void *stream) {
   const char *op = "rkv_pool_append";
   if (!p) return fail(RKV_ERR_INVALID_ARG, op, "pool is NULL");
+  if (rkv_status s = check_q8_pool(p, op)) return s;
   if (layer < 0 || layer >= p->d.layers) return fail(RKV_ERR_INVALID_ARG, op, "layer=%d", layer);
   if (rkv_status s = use_device(p->ctx, op)) return s;
   if (rkv_status s = order_after_last(p, as_stream(stream), op)) return s;
   return rkv_append_q8(p->ctx, &p->g, rkv_pool_layer_pages(p, layer), p->d_tables,
                        p->d.max_pages_per_seq, p->d.max_seqs, args, stream);
+}
+
+rkv_status rkv_pool_append_rope(rkv_pool *p, int32_t layer, const rkv_append_rope_args *args, void *stream) {
+  const char *op = "rkv_pool_append_rope";
+  if (!p) return fail(RKV_ERR_INVALID_ARG, op, "pool is NULL");
+  if (layer < 0 || layer >= p->d.layers) return fail(RKV_ERR_INVALID_ARG, op, "layer=%d", layer);
+  if (args && args->format != p->format)
+    return fail(RKV_ERR_INVALID_ARG, op, "format=%d, the pool's is %d", args->format, p->format);
+  if (rkv_status s = use_device(p->ctx, op)) return s;
+  if (rkv_status s = order_after_last(p, as_stream(stream), op)) return s;
+  return rkv_append_rope(p->ctx, &p->g, rkv_pool_layer_pages(p, layer), p->d_tables,
+                         p->d.max_pages_per_seq, p->d.max_seqs, args, stream);
+}
+
+rkv_status rkv_pool_read_rows(rkv_pool *p, int32_t layer, int32_t n_rows, const int32_t *seq_ids,
+                              const int32_t *positions, void *k_out, void *v_out, int32_t out_dtype,
+                              void *stream) {
+  const char *op = "rkv_pool_read_rows";
+  if (!p) return fail(RKV_ERR_INVALID_ARG, op, "pool is NULL");
+  if (layer < 0 || layer >= p->d.layers) return fail(RKV_ERR_INVALID_ARG, op, "layer=%d", layer);
+  if (rkv_status s = use_device(p->ctx, op)) return s;
+  if (rkv_status s = order_after_last(p, as_stream(stream), op)) return s;
+  return rkv_read_rows(p->ctx, &p->g, p->format, rkv_pool_layer_pages(p, layer), p->d_tables,
+                       p->d.max_pages_per_seq, p->d.max_seqs, n_rows, seq_ids, positions, k_out, v_out,
+                       out_dtype, stream);
 }
 
 rkv_status rkv_pool_decode(rkv_pool *p, int32_t layer, const rkv_decode_args *args, void *stream) {
@@ -1992,6 +2050,9 @@ rkv_status rkv_pool_decode(rkv_pool *p, int32_t layer, const rkv_decode_args *ar
   if (layer < 0 || layer >= p->d.layers) return fail(RKV_ERR_INVALID_ARG, op, "layer=%d", layer);
   if (rkv_status s = use_device(p->ctx, op)) return s;
   if (rkv_status s = order_after_last(p, as_stream(stream), op)) return s;
+  if (p->format == RKV_CACHE_MX4)
+    return rkv_decode_mx4(p->ctx, &p->g, rkv_pool_layer_pages(p, layer), p->d_tables,
+                          p->d.max_pages_per_seq, p->d_lens, p->d.max_seqs, args, stream);
   // pages in host memory: K staged through LDS with V (the register loads
   // of K read the host link at 87% of the LDS-DMA copies' rate)
   return decode_q8(p->ctx, &p->g, rkv_pool_layer_pages(p, layer), p->d_tables,
@@ -2015,6 +2076,9 @@ rkv_status rkv_pool_prefill(rkv_pool *p, int32_t layer, const rkv_prefill_args *
   }
   if (rkv_status s = use_device(p->ctx, op)) return s;
   if (rkv_status s = order_after_last(p, as_stream(stream), op)) return s;
+  if (p->format == RKV_CACHE_MX4)
+    return rkv_prefill_mx4(p->ctx, &p->g, rkv_pool_layer_pages(p, layer), p->d_tables,
+                           p->d.max_pages_per_seq, p->d.max_seqs, args, stream);
   // pages behind the host link: the row blocks of one causal range share
   // one XCD's L2 (in HBM, chunks of 8 spread them over 4 XCDs)
   // (and no widening pass, which would read every page over the link first)
@@ -2026,6 +2090,7 @@ rkv_status rkv_pool_prefill(rkv_pool *p, int32_t layer, const rkv_prefill_args *
 
 size_t rkv_pool_prefill_workspace_bytes(const rkv_pool *p, const rkv_prefill_args *args) {
   if (!p) return 0;
+  if (p->format == RKV_CACHE_MX4) return rkv_prefill_mx4_workspace_bytes(&p->g, args);
   const bool host = p->d.page_memory == RKV_PAGES_HOST;
   return prefill_ws_query(&p->g, args, host ? rkv::kPrefillXcdChunkHost : rkv::kPrefillXcdChunkHbm,
                           !host);
@@ -2035,6 +2100,7 @@ rkv_status rkv_pool_gather(rkv_pool *p, int32_t layer, int32_t seq, int32_t kind
                            void *stream) {
   const char *op = "rkv_pool_gather";
   if (!p) return fail(RKV_ERR_INVALID_ARG, op, "pool is NULL");
+  if (rkv_status s = check_q8_pool(p, op)) return s;
   if (layer < 0 || layer >= p->d.layers) return fail(RKV_ERR_INVALID_ARG, op, "layer=%d", layer);
   if (rkv_status s = check_seq(p->alloc, seq, op)) return s;
   if (rkv_status s = use_device(p->ctx, op)) return s;
@@ -2267,7 +2333,7 @@ rkv_status rkv_r4kv_unpack_host(const uint8_t *page, size_t len, rkv_r4kv_header
 
 size_t rkv_r4kv_page_bytes(const rkv_pool *p, int32_t token_count, int32_t layer_lo,
                            int32_t layer_hi) {
-  if (!p || token_count < 0 || layer_lo < 0 || layer_hi < layer_lo || layer_hi >= p->d.layers)
+  if (!p || p->format != RKV_CACHE_Q8 || token_count < 0 || layer_lo < 0 || layer_hi < layer_lo || layer_hi >= p->d.layers)
     return 0;
   return RKV_R4KV_HEADER_BYTES + spill_body_bytes(p, token_count, layer_hi - layer_lo + 1) + 4;
 }
@@ -2278,6 +2344,7 @@ rkv_status rkv_pool_spill(rkv_pool *p, int32_t seq, int32_t token_start, int32_t
                           void *stream) {
   const char *op = "rkv_pool_spill";
   if (!p) return fail(RKV_ERR_INVALID_ARG, op, "pool is NULL");
+  if (rkv_status s = check_q8_pool(p, op)) return s;
   if (rkv_status s = use_device(p->ctx, op)) return s;
   if (rkv_status s = check_seq(p->alloc, seq, op)) return s;
   if (!identity) return fail(RKV_ERR_INVALID_ARG, op, "identity is NULL");
@@ -2327,6 +2394,7 @@ rkv_status rkv_pool_restore(rkv_pool *p, int32_t seq, const uint8_t *page, size_
   const char *op = "rkv_pool_restore";
   if (refusal) *refusal = RKV_R4KV_ACCEPTED;
   if (!p) return fail(RKV_ERR_INVALID_ARG, op, "pool is NULL");
+  if (rkv_status s = check_q8_pool(p, op)) return s;
   if (rkv_status s = use_device(p->ctx, op)) return s;
   if (rkv_status s = check_seq(p->alloc, seq, op)) return s;
   if (!page || !expect) return fail(RKV_ERR_INVALID_ARG, op, "NULL page/expect");

@@ -125,6 +125,9 @@ __device__ __forceinline__ v8h mx4_v_scales(uint32_t s0, uint32_t s1) {
   return __builtin_bit_cast(v8h, m);
 }
 
+// Bytes of a word of V scales that mark NaN blocks (0x7c and more): their bit 7.
+__device__ __forceinline__ uint32_t mx4_nans(uint32_t s) { return ((s | 0x80808080u) - 0x7c7c7c7cu) & 0x80808080u; }
+
 // Bytes of a word of scales that belong to the first n of its 4 tokens.
 __device__ __forceinline__ uint32_t mx4_keep(int32_t n) { return n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1u; }
 
@@ -187,10 +190,81 @@ __device__ __forceinline__ void mx4_walk(Work &w, Mx4Place &at, int32_t tok, int
     w.template compute<true>(t, tok, tok + step < end ? at.tile<D>(tok + step) : nullptr, at.region);
 }
 
-// G groups of 16 query rows, a row per column, that share the widened K and V
-// of a tile; kTwo: softmax weights of two f16 terms.
+// G groups of 16 query rows, a row per column: their sums and softmax state.
+// kTwo: softmax weights of two f16 terms.
+template <int D, int G, bool kTwo>
+struct Mx4Rows {
+  static constexpr int kTerms = kTwo ? 2 : 1;
+  v4f acc[G][D / 16];  // acc[2b + odd][i]: dim 32*b + 8*lg + 2*i + odd of column li
+  float M[G], l[G];
+  float mul;
+  int32_t rlim[G];     // positions that the lane's row attends
+  int lane, li, lg;
+
+  // The weights of a tile at position tok, from its scores.
+  template <bool kMasked>
+  __device__ __forceinline__ void weights(const v4f (&sc)[G][2], int32_t tok, v8h (&w)[G][kTerms]) {
+    float x[G][8];
+    bool high = false;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const int32_t live = rlim[g] - tok - 8 * lg;
+      float top = kNoMax;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[g][i] = sc[g][i / 4][i % 4];
+        if constexpr (kMasked) x[g][i] = i < live ? x[g][i] : -INFINITY;
+        top = fmaxf(top, x[g][i]);
+      }
+      high = high || __builtin_fmaf(top, mul, -M[g]) > 15.0f;
+    }
+    if (__ballot(high) != 0) rescale(x);
+    const v2h one = {(_Float16)1.0f, (_Float16)1.0f};
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[g][2 * i], mul, -M[g]));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[g][2 * i + 1], mul, -M[g]));
+        const v2h hi = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(p0, p1));
+        w[g][0][2 * i] = hi[0];
+        w[g][0][2 * i + 1] = hi[1];
+        l[g] = __builtin_amdgcn_fdot2(hi, one, l[g], false);
+        if constexpr (kTwo) {
+          const v2h lo = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(p0 - (float)hi[0], p1 - (float)hi[1]));
+          w[g][1][2 * i] = lo[0];
+          w[g][1][2 * i + 1] = lo[1];
+          l[g] = __builtin_amdgcn_fdot2(lo, one, l[g], false);
+        }
+      }
+  }
+
+  // A score outgrew 2^15 over its row's M: the rows' new M puts their largest
+  // at 2^11, and the sums go into its units.
+  __device__ __forceinline__ void rescale(const float (&x)[G][8]) {
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      float top = x[g][0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) top = fmaxf(top, x[g][i]);
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      float n = __builtin_fmaf(top, mul, -11.0f);
+      if (!(n > M[g])) n = M[g];
+      const float f = __builtin_amdgcn_exp2f(M[g] - n);
+      M[g] = n;
+      l[g] *= f;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) acc[g][i] *= f;
+    }
+  }
+};
+
+// G groups of rows that share the widened K and V of a tile.
 template <int D, int G, bool kTwo, bool kBf16>
-struct Mx4Wide {
+struct Mx4Wide : Mx4Rows<D, G, kTwo> {
+  using Rows = Mx4Rows<D, G, kTwo>;
+  using Rows::acc, Rows::rlim, Rows::lane, Rows::lg;
   static constexpr int H = D / 128, NB = D / 32;
   using Query = Mx4Query<D, false, kBf16>;
   static constexpr int kQuery = G * H * 4 * Query::kSets * 64;  // the query operand's 16-byte words in LDS
@@ -199,12 +273,7 @@ struct Mx4Wide {
   // the query operand of (group, half, step, term), 64 lanes' words each
   const __attribute__((address_space(3))) v8b *q;
   __attribute__((address_space(3))) uint8_t *vsc;  // the tile's D bytes of V scales, the wave's own
-  v4f acc[G][D / 16];  // acc[2b + odd][i]: dim 32*b + 8*lg + 2*i + odd of column li
-  float M[G], l[G];
-  float mul;
-  int32_t rlim[G];     // positions that the lane's row attends
-  int32_t end;         // positions that any of the wave's rows attends
-  int lane, li, lg;
+  int32_t end;  // positions that any of the wave's rows attends
 
   // Column li's row of group g (its first element at off, -1: none) into the
   // operand at `to`.
@@ -246,40 +315,8 @@ struct Mx4Wide {
       }
     }
     if (next != nullptr) t.load_k(next, lane);
-    v8h w[G][kTwo ? 2 : 1];
-    float x[G][8];
-    bool high = false;
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-      const int32_t live = rlim[g] - tok - 8 * lg;
-      float top = kNoMax;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[g][i] = sc[g][i / 4][i % 4];
-        if constexpr (kMasked) x[g][i] = i < live ? x[g][i] : -INFINITY;
-        top = fmaxf(top, x[g][i]);
-      }
-      high = high || __builtin_fmaf(top, mul, -M[g]) > 15.0f;
-    }
-    if (__ballot(high) != 0) rescale(x);
-    const v2h one = {(_Float16)1.0f, (_Float16)1.0f};
-#pragma unroll
-    for (int g = 0; g < G; ++g)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[g][2 * i], mul, -M[g]));
-        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[g][2 * i + 1], mul, -M[g]));
-        const v2h hi = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(p0, p1));
-        w[g][0][2 * i] = hi[0];
-        w[g][0][2 * i + 1] = hi[1];
-        l[g] = __builtin_amdgcn_fdot2(hi, one, l[g], false);
-        if constexpr (kTwo) {
-          const v2h lo = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(p0 - (float)hi[0], p1 - (float)hi[1]));
-          w[g][1][2 * i] = lo[0];
-          w[g][1][2 * i + 1] = lo[1];
-          l[g] = __builtin_amdgcn_fdot2(lo, one, l[g], false);
-        }
-      }
+    v8h w[G][Rows::kTerms];
+    Rows::template weights<kMasked>(sc, tok, w);
     mx4_put_scales<D>(vsc, t.vsw, lane);
     const uint32_t keep0 = mx4_keep(end - tok - 8 * lg), keep1 = mx4_keep(end - tok - 8 * lg - 4);
     if constexpr (kMasked) drop_nan(tok, keep0, keep1);
@@ -299,7 +336,7 @@ struct Mx4Wide {
 #pragma unroll
         for (int g = 0; g < G; ++g)
 #pragma unroll
-          for (int k = 0; k < (kTwo ? 2 : 1); ++k)
+          for (int k = 0; k < Rows::kTerms; ++k)
             acc[g][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, w[g][k], acc[g][dt], 0, 0, 0);
       }
     }
@@ -312,15 +349,14 @@ struct Mx4Wide {
   // dims, and the block's scale goes to 0 for the rows that do not (a weight
   // of 0 times NaN is NaN).
   __device__ __forceinline__ void drop_nan(int32_t tok, uint32_t keep0, uint32_t keep1) {
-    auto nans = [](uint32_t s) { return ((s | 0x80808080u) - 0x7c7c7c7cu) & 0x80808080u; };  // bytes of 0x7c and more
     uint32_t any = 0;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) any |= nans(scales(b)[0] & keep0) | nans(scales(b)[1] & keep1);
+    for (int b = 0; b < NB; ++b) any |= mx4_nans(scales(b)[0] & keep0) | mx4_nans(scales(b)[1] & keep1);
     if (__ballot(any != 0) == 0) return;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       const v2u s = scales(b);
-      const uint32_t n0 = nans(s[0] & keep0), n1 = nans(s[1] & keep1);
+      const uint32_t n0 = mx4_nans(s[0] & keep0), n1 = mx4_nans(s[1] & keep1);
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         const int32_t live = rlim[g] - tok - 8 * lg;
@@ -337,26 +373,6 @@ struct Mx4Wide {
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
-  }
-
-  // A score outgrew 2^15 over its row's M: the rows' new M puts their largest
-  // at 2^11, and the sums go into its units.
-  __device__ __forceinline__ void rescale(const float (&x)[G][8]) {
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-      float top = x[g][0];
-#pragma unroll
-      for (int i = 1; i < 8; ++i) top = fmaxf(top, x[g][i]);
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
-      float n = __builtin_fmaf(top, mul, -11.0f);
-      if (!(n > M[g])) n = M[g];
-      const float f = __builtin_amdgcn_exp2f(M[g] - n);
-      M[g] = n;
-      l[g] *= f;
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) acc[g][i] *= f;
-    }
   }
 };
 #endif  // __HIP_DEVICE_COMPILE__

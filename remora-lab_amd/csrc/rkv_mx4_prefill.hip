@@ -17,6 +17,7 @@
 // The scales cost a multiplication per widened V value and none per weight:
 // 64 packed products a tile for all 32 rows at head_dim 256.
 #include <algorithm>
+#include <type_traits>
 
 #include "rkv_mx4_attn.h"
 
@@ -25,10 +26,155 @@ namespace {
 
 constexpr int kMx4PrefillWaves = 4;
 
+#if defined(__HIP_DEVICE_COMPILE__)
+typedef uint8_t __attribute__((address_space(3))) lds_u8;
+
+// A wave's 32 rows of the block, and its part of the widening: D/64 of the
+// tile's D/16 V operands.
+template <int D, bool kTwo>
+struct Mx4Block : Mx4Rows<D, 2, kTwo> {
+  using Rows = Mx4Rows<D, 2, kTwo>;
+  using Rows::acc, Rows::rlim, Rows::lane, Rows::li, Rows::lg;
+  static constexpr int H = D / 128, NB = D / 32, kOwn = D / 64;
+  static constexpr int kOwnBlocks = kOwn / 2;
+
+  v8b q0[2][4];                                    // half 0 of the query operand
+  const __attribute__((address_space(3))) v8b *q1; // half 1, [group][step][lane], the wave's own
+  __attribute__((address_space(3))) v8h *vs;       // [2 tiles][D/16][lane] widened V
+  lds_u8 *nan;                                     // [2 tiles][group of 8 tokens][NB] NaN blocks, a bit a token
+  v4i kc[2 * H];                                   // K codes of (j, h) and their scales
+  uint32_t ks;
+  uint32_t vc[kOwn];                               // the wave's V codes of the next tile,
+  uint32_t vb[2 * kOwnBlocks];                     // and their scales
+  int wave;
+  int32_t whole, end;                              // positions attended by all, and by any, of the block's rows
+
+  __device__ __forceinline__ void load_k(const uint8_t *k) {
+#pragma unroll
+    for (int i = 0; i < 2 * H; ++i) kc[i] = load16_nt(k + 1024 * i + 16 * lane);
+    if constexpr (H == 2) ks = *reinterpret_cast<const uint32_t *>(k + 16 * D + 4 * lane);
+    else ks = *reinterpret_cast<const uint16_t *>(k + 16 * D + 2 * lane);
+  }
+  __device__ __forceinline__ void load_v(const uint8_t *v) {
+    const uint8_t *s = v + 16 * D + 8 * (NB * lg + kOwnBlocks * wave);
+    if constexpr (D == 256) {
+      const v4i c = *reinterpret_cast<const v4i *>(v + 1024 * wave + 16 * lane), x = *reinterpret_cast<const v4i *>(s);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        vc[i] = (uint32_t)c[i];
+        vb[i] = (uint32_t)x[i];
+      }
+    } else {
+      const v2u c = *reinterpret_cast<const v2u *>(v + 1024 * (wave / 2) + 16 * lane + 8 * (wave & 1)),
+                x = *reinterpret_cast<const v2u *>(s);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        vc[i] = c[i];
+        vb[i] = x[i];
+      }
+    }
+  }
+
+  // The wave's part of the tile at tok to LDS.  In a tile that some rows
+  // attend in part, NaN blocks go in as zeros beside their bits (a weight of 0
+  // times NaN is NaN), and tokens behind the block's as zeros.
+  __device__ __forceinline__ void widen(int buf, int32_t tok) {
+    const bool masked = tok + kTile > whole;
+#pragma unroll
+    for (int bb = 0; bb < kOwnBlocks; ++bb) {
+      const int b = kOwnBlocks * wave + bb;
+      uint32_t s0 = vb[2 * bb], s1 = vb[2 * bb + 1];
+      if (masked) {
+        s0 &= mx4_keep(end - tok - 8 * lg);
+        s1 &= mx4_keep(end - tok - 8 * lg - 4);
+        const uint32_t n0 = mx4_nans(s0), n1 = mx4_nans(s1);
+        s0 &= ~((n0 >> 7) * 0xffu);
+        s1 &= ~((n1 >> 7) * 0xffu);
+        auto bits = [](uint32_t n) { return n >> 7 & 1u | n >> 14 & 2u | n >> 21 & 4u | n >> 28 & 8u; };
+        if (li == 0)
+          nan[(4 * buf + lg) * NB + b] = (uint8_t)(bits(n0) | bits(n1) << 4);
+      }
+      const v8h m = mx4_v_scales(s0, s1);
+#pragma unroll
+      for (int odd = 0; odd < 2; ++odd)
+        vs[((D / 16) * buf + 2 * b + odd) * 64 + lane] = mx4_widen_v(vc[2 * bb + odd], 0x1p-2f) * m;  // V times 2^6
+    }
+  }
+
+  // The tile at tok, K in registers and V in buffer buf; the next one's K at
+  // `next` (NULL: none) and the V of the one after it at `after`.
+  template <bool kMasked>
+  __device__ __forceinline__ void compute(int buf, int32_t tok, const uint8_t *next, const uint8_t *after) {
+    // the tile's V is whole, and nobody reads the one before it
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    v4f sc[2][2];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) sc[g][0] = sc[g][1] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        v8b b[2];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) b[g] = h == 0 ? q0[g][u] : q1[(4 * g + u) * 64 + lane];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float scale = __builtin_bit_cast(float, (ks >> (8 * (j * H + h)) & 0xffu) << 23);
+          const v8b a = mx4_widen_k((uint32_t)kc[j * H + h][u], scale);
+#pragma unroll
+          for (int g = 0; g < 2; ++g) sc[g][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[g], sc[g][j], 0, 0, 0);
+        }
+      }
+    if (next != nullptr) {
+      load_k(next);
+      widen(buf ^ 1, tok + kTile);
+      if (after != nullptr) load_v(after);
+    }
+    v8h w[2][Rows::kTerms];
+    Rows::template weights<kMasked>(sc, tok, w);
+    if constexpr (kMasked) add_nan(buf, tok);
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) {
+      const v8h a = vs[((D / 16) * buf + dt) * 64 + lane];
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int k = 0; k < Rows::kTerms; ++k)
+          acc[g][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, w[g][k], acc[g][dt], 0, 0, 0);
+    }
+  }
+
+  // Rows that attend a NaN V block of a masked tile get NaN in its dims.
+  __device__ __forceinline__ void add_nan(int buf, int32_t tok) {
+    const lds_u8 *mine = nan + (4 * buf + lg) * NB;
+    uint32_t any = 0;
+#pragma unroll
+    for (int b = 0; b < NB; b += 4) any |= *reinterpret_cast<const __attribute__((address_space(3))) uint32_t *>(mine + b);
+    if (__ballot(any != 0) == 0) return;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const uint32_t n = mine[b];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const int32_t live = min(max(rlim[g] - tok - 8 * lg, 0), 8);
+        int hit = (n & ((1u << live) - 1u)) != 0u;
+        hit |= __shfl_xor(hit, 16);
+        hit |= __shfl_xor(hit, 32);
+        const float add = hit ? __builtin_nanf("") : 0.0f;
+        acc[g][2 * b] += add;
+        acc[g][2 * b + 1] += add;
+      }
+    }
+  }
+};
+#endif  // __HIP_DEVICE_COMPILE__
+
 template <int D, bool kTwo>
 __global__ __launch_bounds__(64 * kMx4PrefillWaves, 2) void mx4_prefill_kernel(PrefillLaunch pf) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  using Pre = Mx4Wide<D, 2, kTwo, true>;
+  using Pre = Mx4Block<D, kTwo>;
   const DecodeLaunch &p = pf.d;
   // the workgroup's unit (see prefill_kernel)
   const uint32_t C = (uint32_t)max(pf.xcd_chunk, 1);
@@ -54,13 +200,15 @@ __global__ __launch_bounds__(64 * kMx4PrefillWaves, 2) void mx4_prefill_kernel(P
   const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
   const int r0 = 32 * (int)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int32_t G = p.q_heads / heads;
-  if (r0 / G >= jn) return;  // (waves share nothing: no barrier waits for this one)
 
-  __shared__ v8b qs[kMx4PrefillWaves][Pre::kQuery];
+  __shared__ v8h vs[2][D / 16][64];
+  __shared__ v8b qs[kMx4PrefillWaves][D == 256 ? 2 * 4 * 64 : 1];
+  __shared__ uint32_t nans[2][4][Pre::NB / 4];
   Pre pr;
-  __shared__ __attribute__((aligned(16))) uint8_t vscs[kMx4PrefillWaves][D];
-  pr.q = (const __attribute__((address_space(3))) v8b *)qs[r0 / 32];
-  pr.vsc = (__attribute__((address_space(3))) uint8_t *)vscs[r0 / 32];
+  pr.vs = (__attribute__((address_space(3))) v8h *)&vs[0][0][0];
+  pr.q1 = (const __attribute__((address_space(3))) v8b *)qs[r0 / 32];
+  pr.nan = (lds_u8 *)&nans[0][0][0];
+  pr.wave = r0 / 32;
   pr.lane = lane;
   pr.li = li;
   pr.lg = lg;
@@ -70,20 +218,44 @@ __global__ __launch_bounds__(64 * kMx4PrefillWaves, 2) void mx4_prefill_kernel(P
     const int r = r0 + 16 * c + li, jl = r / G;
     const int64_t off =
         jl < jn ? ((int64_t)(pf.qoff[e] + j0 + jl) * p.q_heads + kvh * G + r % G) * D : -1;
-    pr.put_query(qs[r0 / 32], c, p.q, off, p.scale_log2 < 0.0f ? -1.0f : 1.0f);
+    Mx4Query<D, false, true> x;
+    x.load(p.q, off, p.scale_log2 < 0.0f ? -1.0f : 1.0f, false, lg);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      pr.q0[c][u] = x.b[0][0][u];
+      if constexpr (D == 256) qs[r0 / 32][(4 * c + u) * 64 + lane] = x.b[0][1][u];
+    }
     pr.rlim[c] = jl < jn ? ctx + j0 + jl + 1 : 0;
     pr.M[c] = kNoMax;
     pr.l[c] = 0.0f;
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) pr.acc[c][i] = v4f{0.f, 0.f, 0.f, 0.f};
   }
-  // positions attended by all, and by any, of the wave's rows
-  const int32_t all = ctx + j0 + r0 / G + 1;
-  pr.end = ctx + j0 + min((r0 + 31) / G, jn - 1) + 1;
-  const int32_t last = min(tok_end, pr.end);
+  pr.whole = ctx + j0 + 1;
+  pr.end = len;
 
+  // every wave walks every tile of the block; a tile's V is widened while the
+  // one before it is worked on
   Mx4Place at(p, seq, kvh);
-  mx4_walk<D>(pr, at, tok0, kTile, min(all, last), last, [] {});
+  if (tok0 < tok_end) {
+    const uint8_t *k = at.tile<D>(tok0);
+    pr.load_k(k);
+    pr.load_v(k + at.region);
+    const uint8_t *next = tok0 + kTile < tok_end ? at.tile<D>(tok0 + kTile) : nullptr;
+    pr.widen(0, tok0);
+    if (next != nullptr) pr.load_v(next + at.region);
+    int buf = 0;
+    int32_t tok = tok0;
+    auto step = [&](auto masked) {
+      const uint8_t *after = tok + 2 * kTile < tok_end ? at.tile<D>(tok + 2 * kTile) : nullptr;
+      pr.template compute<decltype(masked)::value>(buf, tok, next, after != nullptr ? after + at.region : nullptr);
+      next = after;
+      buf ^= 1;
+      tok += kTile;
+    };
+    while (tok < tok_end && tok + kTile <= pr.whole) step(std::false_type{});
+    while (tok < tok_end) step(std::true_type{});
+  }
   if (at.bad && lane == 0) atomicOr(p.fault, FAULT_BAD_PAGE);
 
 #pragma unroll

@@ -219,6 +219,8 @@ struct Mx4Rows {
       high = high || __builtin_fmaf(top, mul, -M[g]) > 15.0f;
     }
     if (__ballot(high) != 0) rescale(x);
+    float minus = -1.0f;
+    asm("" : "+s"(minus));  // (a factor to the compiler: one mixed fma and not a conversion and a difference)
     const v2h one = {(_Float16)1.0f, (_Float16)1.0f};
 #pragma unroll
     for (int g = 0; g < G; ++g)
@@ -231,7 +233,8 @@ struct Mx4Rows {
         w[g][0][2 * i + 1] = hi[1];
         l[g] = __builtin_amdgcn_fdot2(hi, one, l[g], false);
         if constexpr (kTwo) {
-          const v2h lo = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(p0 - (float)hi[0], p1 - (float)hi[1]));
+          const v2h lo = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(
+              __builtin_fmaf((float)hi[0], minus, p0), __builtin_fmaf((float)hi[1], minus, p1)));
           w[g][1][2 * i] = lo[0];
           w[g][1][2 * i + 1] = lo[1];
           l[g] = __builtin_amdgcn_fdot2(lo, one, l[g], false);

@@ -135,14 +135,24 @@ struct Mx4Block : Mx4Rows<D, 2, kTwo> {
     v8h w[2][Rows::kTerms];
     Rows::template weights<kMasked>(sc, tok, w);
     if constexpr (kMasked) add_nan(buf, tok);
+    // each step's V operands are on their way during the step before
+    v8h a[2][2];
+    auto load = [&](int s) {
 #pragma unroll
-    for (int dt = 0; dt < D / 16; ++dt) {
-      const v8h a = vs[((D / 16) * buf + dt) * 64 + lane];
+      for (int i = 0; i < 2; ++i) a[s & 1][i] = vs[((D / 16) * buf + 2 * s + i) * 64 + lane];
+    };
+    load(0);
 #pragma unroll
-      for (int g = 0; g < 2; ++g)
+    for (int s = 0; s < NB; ++s) {
+      if (s + 1 < NB) load(s + 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int k = 0; k < Rows::kTerms; ++k)
-          acc[g][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, w[g][k], acc[g][dt], 0, 0, 0);
+      for (int k = 0; k < Rows::kTerms; ++k)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int g = 0; g < 2; ++g)
+            acc[g][2 * s + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[s & 1][i], w[g][k], acc[g][2 * s + i], 0, 0, 0);
     }
   }
 
@@ -172,7 +182,7 @@ struct Mx4Block : Mx4Rows<D, 2, kTwo> {
 #endif  // __HIP_DEVICE_COMPILE__
 
 template <int D, bool kTwo>
-__global__ __launch_bounds__(64 * kMx4PrefillWaves, 2) void mx4_prefill_kernel(PrefillLaunch pf) {
+__global__ __launch_bounds__(64 * kMx4PrefillWaves, D == 128 ? 3 : 2) void mx4_prefill_kernel(PrefillLaunch pf) {
 #if defined(__HIP_DEVICE_COMPILE__)
   using Pre = Mx4Block<D, kTwo>;
   const DecodeLaunch &p = pf.d;

@@ -12,6 +12,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <functional>
+#include <limits>
 #include <string>
 #include <thread>
 #include <vector>
@@ -857,6 +858,73 @@ int64_t simulate_prefill(const int32_t *ctx, const int32_t *rows, const int32_t 
   return *std::max_element(load.begin(), load.end());
 }
 
+// The same of rkv_prefill_mx4, whose workgroups share a CU two at a time, each
+// at full rate, and run 1.4 times as fast alone (equal units of 2.5 to 220
+// tiles, 128 to 2048 a launch: 2.0 us a tile in pairs, 1.4 alone, and as much
+// as 8 tiles for a unit's queries and rows, half as much again for split
+// ones).  Tokens of a paired workgroup; a split adds its combine: a launch and
+// its rows' partials read.  Measured against it, six chunks of 173..567 rows
+// after 422..2954 tokens: segments of 2048 tokens 155 us for 2741 + 0, none
+// 173 for 3282, 1024 181 for 3389, 512 230 for 4463.
+constexpr double kPairUnit = 256, kPairSplitUnit = 128, kPairAlone = 1.4, kPairCombine = 96, kPairRows = 1.0 / 300;
+
+int64_t simulate_pairs(const int32_t *ctx, const int32_t *rows, const int32_t *order, int32_t n,
+                       int32_t tq, int32_t kv_heads, int64_t seg, int32_t xcd_chunk, int64_t partial_rows) {
+  constexpr int kXcds = 8;
+  constexpr int kCus = rkv::kComputeUnits / kXcds;
+  struct Cu {
+    double left[2] = {0, 0};  // of its workgroups, in tokens
+    int held = 0;
+    double now = 0, done = std::numeric_limits<double>::infinity();  // the first to end
+    double rate() const { return held == 2 ? 1.0 : kPairAlone; }
+    void go(double t) {
+      for (int i = 0; i < held; ++i) left[i] -= (t - now) * rate();
+      now = t;
+    }
+    void next() {
+      done = held == 0 ? std::numeric_limits<double>::infinity()
+                       : now + (held == 2 ? std::min(left[0], left[1]) : left[0]) / rate();
+    }
+  };
+  Cu cus[kXcds][kCus];
+  int started[kXcds] = {};
+  double end = 0;
+  auto finish = [&](Cu *x) {  // the XCD's next workgroup to end; its CU
+    Cu *c = std::min_element(x, x + kCus, [](const Cu &a, const Cu &b) { return a.done < b.done; });
+    c->go(c->done);
+    if (c->held == 2 && c->left[0] <= c->left[1]) c->left[0] = c->left[1];
+    --c->held;
+    c->next();
+    return c;
+  };
+  int64_t j = 0;
+  for (int32_t k = 0; k < n; ++k) {
+    const int64_t c = ctx[order[k]], r = rows[order[k]];
+    const int64_t nb = (r + tq - 1) / tq;
+    const int32_t ns = segments_of(c + r, (int32_t)seg);
+    for (int32_t sg = 0; sg < ns; ++sg)
+      for (int32_t h = 0; h < kv_heads; ++h)
+        for (int64_t b = nb - 1; b >= 0; --b, ++j) {
+          const int64_t range = c + std::min<int64_t>(tq * (b + 1), r);
+          const int64_t len = ns == 1 ? range : std::clamp<int64_t>(range - sg * seg, 0, seg);
+          const int x = (int)(j / xcd_chunk % kXcds);
+          Cu *cu = started[x] < 2 * kCus ? &cus[x][started[x]++ % kCus] : finish(cus[x]);
+          cu->left[cu->held++] = (double)len + kPairUnit + (ns > 1 ? kPairSplitUnit : 0);
+          cu->next();
+        }
+  }
+  for (auto &x : cus)
+    for (Cu &c : x)
+      while (c.held > 0) {
+        end = std::max(end, c.done);
+        c.go(c.done);
+        if (c.held == 2 && c.left[0] <= c.left[1]) c.left[0] = c.left[1];
+        --c.held;
+        c.next();
+      }
+  return (int64_t)(end + (partial_rows > 0 ? kPairCombine + (double)partial_rows * kPairRows : 0));
+}
+
 // The automatic split.  A launch whose units do not divide evenly over the
 // CUs -- too few row blocks, or a few long causal ranges among short ones --
 // ends when its longest units do; cutting every range longer than a segment
@@ -866,12 +934,13 @@ int64_t simulate_prefill(const int32_t *ctx, const int32_t *rows, const int32_t 
 template <typename RowsFor>
 SegPlan auto_segments(const rkv_kv_geometry *g, int32_t q_heads, int32_t tq, int32_t n,
                       const int32_t *ctx_lens, const int32_t *q_rows, size_t cap,
-                      int32_t xcd_chunk, int64_t max_range, int64_t seg_floor, RowsFor rows_for) {
+                      int32_t xcd_chunk, bool mx4, int64_t max_range, int64_t seg_floor,
+                      RowsFor rows_for) {
   SegPlan none;
   thread_local std::vector<int64_t> memo_key;
   thread_local SegPlan memo_plan;
   std::vector<int64_t> key = {tq, q_heads, g->kv_heads, g->page_tokens, g->head_dim,
-                              (int64_t)std::min<size_t>(cap, INT64_MAX), xcd_chunk, n};
+                              (int64_t)std::min<size_t>(cap, INT64_MAX), xcd_chunk, mx4, n};
   for (int32_t e = 0; e < n; ++e) {
     key.push_back(ctx_lens[e]);
     key.push_back(q_rows[e]);
@@ -891,11 +960,18 @@ SegPlan auto_segments(const rkv_kv_geometry *g, int32_t q_heads, int32_t tq, int
   if (units > 0 && units * g->kv_heads <= kMaxSimUnits / 4) {
     const int64_t unit = std::max<int32_t>(32, g->page_tokens);
     auto round_up = [&](int64_t t) { return (t + unit - 1) / unit * unit; };
-    const int64_t base = simulate_prefill(ctx_lens, q_rows, order, n, tq, g->kv_heads, 0, xcd_chunk);
+    auto simulate = [&](int64_t seg, int64_t partial_rows) {
+      return mx4 ? simulate_pairs(ctx_lens, q_rows, order, n, tq, g->kv_heads, seg, xcd_chunk, partial_rows)
+                 : simulate_prefill(ctx_lens, q_rows, order, n, tq, g->kv_heads, seg, xcd_chunk);
+    };
+    const int64_t base = simulate(0, 0);
     int64_t best_t = base;
     int64_t last = -1;
-    for (int64_t k : {2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
-      const int64_t seg = std::max<int64_t>({round_up((max_range + k - 1) / k),
+    // (in eighths; 4-bit pages below two segments too, where a few ranges are
+    // longer than the rest)
+    for (int64_t k : {10, 12, 13, 14, 15, 16, 20, 24, 32, 48, 64, 96, 128, 192, 256, 384, 512}) {
+      if (!mx4 && (k < 16 || k == 20)) continue;
+      const int64_t seg = std::max<int64_t>({round_up((8 * max_range + k - 1) / k),
                                              round_up(kPrefillMinSegment), seg_floor});
       if (seg >= max_range || seg == last) continue;
       last = seg;
@@ -906,7 +982,7 @@ SegPlan auto_segments(const rkv_kv_geometry *g, int32_t q_heads, int32_t tq, int
       if (su * g->kv_heads > kMaxSimUnits) continue;
       const int64_t p = rows_for(seg);
       if (p == 0 || prefill_ws_bytes(p, g->head_dim) > cap) continue;
-      const int64_t t = simulate_prefill(ctx_lens, q_rows, order, n, tq, g->kv_heads, seg, xcd_chunk);
+      const int64_t t = simulate(seg, p);
       if (t < best_t) {
         best_t = t;
         best.seg = (int32_t)seg;
@@ -923,7 +999,7 @@ SegPlan auto_segments(const rkv_kv_geometry *g, int32_t q_heads, int32_t tq, int
 // cap: workspace bytes available to the automatic split.
 SegPlan plan_segments(const rkv_kv_geometry *g, int32_t q_heads, int32_t tq, int32_t n,
                       const int32_t *ctx_lens, const int32_t *q_rows, int32_t request,
-                      size_t cap, int32_t xcd_chunk) {
+                      size_t cap, int32_t xcd_chunk, bool mx4) {
   SegPlan none;
   if (request < 0 || n <= 0) return none;
   const int64_t unit = std::max<int32_t>(32, g->page_tokens);
@@ -949,7 +1025,7 @@ SegPlan plan_segments(const rkv_kv_geometry *g, int32_t q_heads, int32_t tq, int
   }
   // automatic: simulate the launch for a few segment lengths and keep the
   // shortest makespan, if it beats the unsplit launch by a twentieth
-  return auto_segments(g, q_heads, tq, n, ctx_lens, q_rows, cap, xcd_chunk, max_range, seg_floor,
+  return auto_segments(g, q_heads, tq, n, ctx_lens, q_rows, cap, xcd_chunk, mx4, max_range, seg_floor,
                        rows_for);
 }
 
@@ -959,7 +1035,7 @@ SegPlan plan_segments(const rkv_kv_geometry *g, int32_t q_heads, int32_t tq, int
 rkv_status make_prefill(rkv_ctx *ctx, const rkv_kv_geometry *g, const void *pages,
                         const int32_t *bt, int32_t bt_stride, int32_t n_seqs,
                         const rkv_prefill_args *a, const char *op, int32_t xcd_chunk,
-                        bool widen_once, rkv::PrefillLaunch &pf) {
+                        bool widen_once, bool mx4, rkv::PrefillLaunch &pf) {
   if (rkv_status s = check_geometry(g, op)) return s;
   if (rkv_status s = check_tables(pages, bt, bt_stride, n_seqs, op)) return s;
   if (!a) return fail(RKV_ERR_INVALID_ARG, op, "args is NULL");
@@ -1003,7 +1079,7 @@ rkv_status make_prefill(rkv_ctx *ctx, const rkv_kv_geometry *g, const void *page
     return fail(RKV_ERR_INVALID_ARG, op, "workspace is not 256-byte aligned");
   const SegPlan sp = plan_segments(g, a->q_heads, pf.tq, a->n_seqs, a->ctx_lens, a->q_rows,
                                    a->segment_tokens, a->workspace ? a->workspace_bytes : 0,
-                                   xcd_chunk);
+                                   xcd_chunk, mx4);
   const size_t ws_need = prefill_ws_bytes(sp.partial_rows, g->head_dim);
   if (ws_need > 0 && (!a->workspace || a->workspace_bytes < ws_need))
     return fail(RKV_ERR_INVALID_ARG, op, "segment_tokens=%d needs a %zu-byte workspace (have %zu)",
@@ -1092,7 +1168,7 @@ rkv_status prefill_q8(rkv_ctx *ctx, const rkv_kv_geometry *g, const void *pages,
   if (rkv_status s = use_device(ctx, op)) return s;
   rkv::PrefillLaunch pf{};
   if (rkv_status s =
-          make_prefill(ctx, g, pages, block_tables, bt_stride, n_seqs, a, op, xcd_chunk, widen_once, pf))
+          make_prefill(ctx, g, pages, block_tables, bt_stride, n_seqs, a, op, xcd_chunk, widen_once, false, pf))
     return s;
   hipError_t e = rkv::launch_prefill(pf, as_stream(stream));
   return e == hipSuccess ? RKV_OK : hip_fail(op, e);
@@ -1118,7 +1194,7 @@ constexpr int32_t kMx4PrefillXcdChunk = rkv::kPrefillXcdChunkHbm;
 // dispatch simulation depends on it), with room for the widened tiles when
 // the launch would widen once (HBM pages and a bf16 query).
 size_t prefill_ws_query(const rkv_kv_geometry *g, const rkv_prefill_args *a, int32_t xcd_chunk,
-                        bool widen_once) {
+                        bool widen_once, bool mx4 = false) {
   if (!g || !a || check_geometry(g, "rkv_prefill_workspace_bytes") != RKV_OK) return 0;
   if (a->n_seqs < 1 || a->n_seqs > RKV_PREFILL_MAX_SEQS || !a->ctx_lens || !a->q_rows) return 0;
   if (a->q_heads < 1 || a->q_heads % g->kv_heads != 0) return 0;
@@ -1127,7 +1203,7 @@ size_t prefill_ws_query(const rkv_kv_geometry *g, const rkv_prefill_args *a, int
   for (int32_t e = 0; e < a->n_seqs; ++e)
     if (a->ctx_lens[e] < 0 || a->q_rows[e] < 0) return 0;
   const SegPlan sp = plan_segments(g, a->q_heads, rkv::kPrefillRows / G, a->n_seqs, a->ctx_lens,
-                                   a->q_rows, a->segment_tokens, SIZE_MAX, xcd_chunk);
+                                   a->q_rows, a->segment_tokens, SIZE_MAX, xcd_chunk, mx4);
   const size_t partials = prefill_ws_bytes(sp.partial_rows, g->head_dim);
   if (a->q_dtype != RKV_BF16 || !widen_once) return partials;
   return prefill_pre_at(partials) + prefill_pre_bytes(g, a->n_seqs, a->ctx_lens, a->q_rows);
@@ -1138,7 +1214,7 @@ extern "C" {
 
 size_t rkv_prefill_mx4_workspace_bytes(const rkv_kv_geometry *g, const rkv_prefill_args *a) {
   if (check_mx4_geometry(g, "rkv_prefill_mx4_workspace_bytes") != RKV_OK) return 0;
-  return prefill_ws_query(g, a, kMx4PrefillXcdChunk, false);
+  return prefill_ws_query(g, a, kMx4PrefillXcdChunk, false, true);
 }
 
 rkv_status rkv_prefill_mx4(rkv_ctx *ctx, const rkv_kv_geometry *g, const void *pages,
@@ -1147,7 +1223,7 @@ rkv_status rkv_prefill_mx4(rkv_ctx *ctx, const rkv_kv_geometry *g, const void *p
   const char *op = "rkv_prefill_mx4";
   if (rkv_status s = check_mx4_geometry(g, op)) return s;
   rkv::PrefillLaunch pf{};
-  if (rkv_status s = make_prefill(ctx, g, pages, block_tables, bt_stride, n_seqs, a, op, kMx4PrefillXcdChunk, false, pf))
+  if (rkv_status s = make_prefill(ctx, g, pages, block_tables, bt_stride, n_seqs, a, op, kMx4PrefillXcdChunk, false, true, pf))
     return s;
   if (a->q_dtype != RKV_BF16) return fail(RKV_ERR_UNSUPPORTED, op, "q_dtype=%d (built for 4-bit pages: bf16)", a->q_dtype);
   if (rkv_status s = use_device(ctx, op)) return s;

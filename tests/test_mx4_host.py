@@ -112,3 +112,26 @@ def test_prefill_refusals(rkv, over, status, text):
 def test_prefill_refuses_small_pages(rkv):
     st, msg = _prefill(rkv, rkv.geometry(2, 256, 16, 10))
     assert st == -4 and "page_tokens=16" in msg
+
+
+def test_prefill_plan(rkv):
+    """The split that rkv_prefill_mx4 plans, by its workspace: (m, l) rows padded
+    to 256 bytes and o rows, rows * q_heads * segments of the entries that split."""
+    import torch
+
+    def rows(entries, G, kv, PT, seg=0):
+        g = rkv.geometry(kv, 256, PT, 1 << 20)
+        q = torch.empty(sum(r for _, r in entries), G * kv, 256, dtype=torch.bfloat16)
+        a = rkv.prefill_args(list(range(len(entries))), [c for c, _ in entries], [r for _, r in entries], q, q, 1.0,
+                             segment_tokens=seg)
+        return rkv.prefill_mx4_workspace_bytes(g, a)
+
+    def need(p):
+        return (p * 8 + 255) // 256 * 256 + p * 1024
+    assert rows([(8192, 512)] * 8, 8, 2, 64) == 0           # two equal units a CU
+    assert rows([(0, 4096)], 8, 2, 64) == 0
+    assert rows([(32768, 512)], 8, 2, 64, seg=-1) == 0
+    assert rows([(32768, 512)], 8, 2, 64) == need(512 * 16 * 8)  # 64 units: 8 segments each, two a CU
+    # among shorter ranges only the longest are cut, in two
+    mixed = [(966, 173), (1242, 269), (422, 328), (2954, 567), (1622, 267), (1961, 526)]
+    assert rows(mixed, 6, 4, 32) == need(24 * 2 * (567 + 526 + 267)) or rows(mixed, 6, 4, 32) == need(24 * 2 * (567 + 526))

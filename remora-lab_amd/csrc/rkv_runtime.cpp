@@ -925,6 +925,17 @@ int64_t simulate_pairs(const int32_t *ctx, const int32_t *rows, const int32_t *o
   return (int64_t)(end + (partial_rows > 0 ? kPairCombine + (double)partial_rows * kPairRows : 0));
 }
 
+int64_t pairs_mean(const int32_t *ctx, const int32_t *rows, int32_t n, int32_t tq, int32_t kv_heads, int64_t seg) {
+  double sum = 0;
+  for (int32_t e = 0; e < n; ++e) {
+    const int64_t c = ctx[e], r = rows[e], nb = (r + tq - 1) / tq;
+    const int32_t ns = segments_of(c + r, (int32_t)seg);
+    for (int64_t b = 0; b < nb; ++b) sum += (double)(c + std::min<int64_t>(tq * (b + 1), r));
+    sum += (double)(nb * ns) * (kPairUnit + (ns > 1 ? kPairSplitUnit : 0));
+  }
+  return (int64_t)(sum * kv_heads / (2 * rkv::kComputeUnits));
+}
+
 // The automatic split.  A launch whose units do not divide evenly over the
 // CUs -- too few row blocks, or a few long causal ranges among short ones --
 // ends when its longest units do; cutting every range longer than a segment
@@ -980,6 +991,8 @@ SegPlan auto_segments(const rkv_kv_geometry *g, int32_t q_heads, int32_t tq, int
         su += ((int64_t)q_rows[e] + tq - 1) / tq *
               segments_of((int64_t)ctx_lens[e] + q_rows[e], (int32_t)seg);
       if (su * g->kv_heads > kMaxSimUnits) continue;
+      // (no order makes a launch shorter than its slots' mean load)
+      if (mx4 && pairs_mean(ctx_lens, q_rows, n, tq, g->kv_heads, seg) * 20 > base * 19) continue;
       const int64_t p = rows_for(seg);
       if (p == 0 || prefill_ws_bytes(p, g->head_dim) > cap) continue;
       const int64_t t = simulate(seg, p);

@@ -344,13 +344,14 @@ size_t rkv_prefill_workspace_bytes(const rkv_kv_geometry *g, const rkv_prefill_a
  * bytes a block.  e is the smallest exponent with max|v| <= 7 * 2^e, kept
  * within -24..15 for K and -22..7 for V; a code is v / 2^e rounded to nearest,
  * ties to the even code, saturating at 6.  A block with a value that is not
- * finite reads back as NaN.  Pages have the geometry, allocator and block tables
- * of the Q8_0 ones, with page_tokens 32, 64, 128 or 256 and rkv_mx4_page_bytes
- * bytes, in device memory; their layout is internal (rkv_append_rope writes
- * and rkv_read_rows reads them).  A pool holds them with
- * rkv_pool_create_format.  No counterpart in the reference,
- * whose flash decode reads Q8_0 only (har/shaders/flash_decode_q8.comp:1-25);
- * har/crates/r4kv's own 4-bit format packs integer codes under an f16 scale. */
+ * finite reads back as NaN.  Pages have the geometry, allocator and block
+ * tables of the Q8_0 ones, with page_tokens 32, 64, 128 or 256 and
+ * rkv_mx4_page_bytes bytes, in device memory at a multiple of 16 bytes; their
+ * layout is internal (rkv_append_rope writes and rkv_read_rows reads them).
+ * A pool holds them with rkv_pool_create_format.  No counterpart in the
+ * reference, whose flash decode reads Q8_0 only
+ * (har/shaders/flash_decode_q8.comp:1-25); har/crates/r4kv's own 4-bit format
+ * packs integer codes under an f16 scale. */
 size_t rkv_mx4_page_bytes(const rkv_kv_geometry *g);
 /* rkv_copy_pages of 4-bit pages. */
 rkv_status rkv_mx4_copy_pages(rkv_ctx *ctx, const rkv_kv_geometry *g, void *pages,
@@ -410,7 +411,7 @@ typedef struct rkv_rope_args {
 } rkv_rope_args;
 
 typedef struct rkv_rope_rows_args {
-  int32_t n_rows;
+  int32_t n_rows;           /* up to 2^23 */
   int32_t head_dim;         /* 128 or 256 */
   int32_t q_heads;          /* 0: no queries */
   int32_t kv_heads;         /* 0: no keys */
@@ -434,7 +435,7 @@ rkv_status rkv_rope_rows(rkv_ctx *ctx, const rkv_rope_args *rope, const rkv_rope
 
 enum { RKV_CACHE_Q8 = 0, RKV_CACHE_MX4 = 1 };  /* page formats */
 typedef struct rkv_append_rope_args {
-  int32_t n_rows;
+  int32_t n_rows;           /* up to 2^23 */
   const int32_t *seq_ids;   /* device [n_rows] */
   const int32_t *positions; /* device [n_rows], token index within the sequence; a
                                sequence's position appears once in a call */
@@ -458,17 +459,19 @@ typedef struct rkv_append_rope_args {
  * are) on the way, and the rows' queries beside.  Keys are normed and rotated
  * in f64 and rounded to f32 once; from there a Q8 row has the bytes that
  * rkv_append_q8 gives it.  With rope NULL and format Q8 it is rkv_append_q8 of
- * strided rows.  Sources, q_out and strides are multiples of 16 bytes.  Faults
- * as in rkv_append_q8; their rows are not written (their queries are).  Calls
- * that overlap must not append to the same 8 tokens (4 with Q8) of a sequence. */
+ * strided rows.  Pages, sources, q_out and strides are multiples of 16 bytes.
+ * Faults as in rkv_append_q8; their rows are not written (their queries are).
+ * Calls that overlap must not append to the same 8 tokens (4 with Q8) of a
+ * sequence. */
 rkv_status rkv_append_rope(rkv_ctx *ctx, const rkv_kv_geometry *g, void *pages,
                            const int32_t *block_tables, int32_t bt_stride, int32_t n_seqs,
                            const rkv_append_rope_args *args, void *stream);
 
 /* The values of cached rows, code times scale (an 8-bit one's in f32): k_out
- * and v_out [n_rows][kv_heads][head_dim], either may be NULL, 16-byte aligned.
- * Rows that name no slot are reported as in rkv_append_q8 and read as 0.  (The
- * reference's q8_0_dequant_row, attention.rs:79-90, a row at a time.) */
+ * and v_out [n_rows][kv_heads][head_dim], either may be NULL, at multiples of
+ * 16 bytes like the pages; up to 2^23 rows.  Rows that name no slot are reported
+ * as in rkv_append_q8 and read as 0.  (The reference's q8_0_dequant_row,
+ * attention.rs:79-90, a row at a time.) */
 rkv_status rkv_read_rows(rkv_ctx *ctx, const rkv_kv_geometry *g, int32_t format, const void *pages,
                          const int32_t *block_tables, int32_t bt_stride, int32_t n_seqs,
                          int32_t n_rows, const int32_t *seq_ids, const int32_t *positions,

@@ -774,6 +774,13 @@ rkv_status check_tables(const void *pages, const int32_t *bt, int32_t bt_stride,
     return fail(RKV_ERR_INVALID_ARG, op, "bt_stride=%d n_seqs=%d", bt_stride, n_seqs);
   return RKV_OK;
 }
+// of the calls that read or write whole 16-byte words of a page
+rkv_status check_whole_words(const void *pages, const int32_t *bt, int32_t bt_stride, int32_t n_seqs, const char *op) {
+  if (rkv_status s = check_tables(pages, bt, bt_stride, n_seqs, op)) return s;
+  if (reinterpret_cast<uintptr_t>(pages) % 16 != 0)
+    return fail(RKV_ERR_INVALID_ARG, op, "pages must be a multiple of 16 bytes");
+  return RKV_OK;
+}
 
 rkv::AppendLaunch make_append(rkv_ctx *ctx, const rkv_kv_geometry *g, void *pages, const int32_t *block_tables,
                               int32_t bt_stride, int32_t n_seqs, int32_t n_rows, const int32_t *seq_ids,
@@ -1235,6 +1242,7 @@ rkv_status rkv_prefill_mx4(rkv_ctx *ctx, const rkv_kv_geometry *g, const void *p
                            const rkv_prefill_args *a, void *stream) {
   const char *op = "rkv_prefill_mx4";
   if (rkv_status s = check_mx4_geometry(g, op)) return s;
+  if (rkv_status s = check_whole_words(pages, block_tables, bt_stride, n_seqs, op)) return s;
   rkv::PrefillLaunch pf{};
   if (rkv_status s = make_prefill(ctx, g, pages, block_tables, bt_stride, n_seqs, a, op, kMx4PrefillXcdChunk, false, true, pf))
     return s;
@@ -1279,6 +1287,9 @@ rkv_status rkv_append_q8(rkv_ctx *ctx, const rkv_kv_geometry *g, void *pages,
 
 namespace {
 // Rows of `heads` heads: a pointer and a stride that 16-byte accesses fit.
+constexpr int32_t kMaxRows = 1 << 23;   // of a call: every grid stays within 2^31 threads
+constexpr int32_t kMaxHeads = 1 << 14;  // (a grid's y)
+
 rkv_status check_head_rows(const void *p, int64_t stride, int32_t heads, int32_t head_dim, bool bf16,
                            const char *what, const char *op) {
   if (!p) return fail(RKV_ERR_INVALID_ARG, op, "%s is NULL", what);
@@ -1346,7 +1357,8 @@ rkv_status rkv_rope_rows(rkv_ctx *ctx, const rkv_rope_args *rope, const rkv_rope
   if (!rope || !a) return fail(RKV_ERR_INVALID_ARG, op, "NULL argument");
   if (a->head_dim != 128 && a->head_dim != 256)
     return fail(RKV_ERR_UNSUPPORTED, op, "head_dim=%d (built: 128, 256)", a->head_dim);
-  if (a->n_rows < 0 || a->q_heads < 0 || a->kv_heads < 0)
+  if (a->n_rows < 0 || a->n_rows > kMaxRows || a->q_heads < 0 || a->kv_heads < 0 || a->q_heads > kMaxHeads ||
+      a->kv_heads > kMaxHeads)
     return fail(RKV_ERR_INVALID_ARG, op, "n_rows=%d q_heads=%d kv_heads=%d", a->n_rows, a->q_heads, a->kv_heads);
   if (!dtype_ok(a->src_dtype) || !dtype_ok(a->out_dtype))
     return fail(RKV_ERR_UNSUPPORTED, op, "src_dtype=%d out_dtype=%d", a->src_dtype, a->out_dtype);
@@ -1377,8 +1389,8 @@ rkv_status rkv_append_rope(rkv_ctx *ctx, const rkv_kv_geometry *g, void *pages, 
   const char *op = "rkv_append_rope";
   if (!a) return fail(RKV_ERR_INVALID_ARG, op, "args is NULL");
   if (rkv_status s = check_format(g, a->format, op)) return s;
-  if (rkv_status s = check_tables(pages, block_tables, bt_stride, n_seqs, op)) return s;
-  if (a->n_rows < 0) return fail(RKV_ERR_INVALID_ARG, op, "n_rows=%d", a->n_rows);
+  if (rkv_status s = check_whole_words(pages, block_tables, bt_stride, n_seqs, op)) return s;
+  if (a->n_rows < 0 || a->n_rows > kMaxRows) return fail(RKV_ERR_INVALID_ARG, op, "n_rows=%d", a->n_rows);
   if (!dtype_ok(a->src_dtype)) return fail(RKV_ERR_UNSUPPORTED, op, "src_dtype=%d", a->src_dtype);
   if (a->rule != 0 && !(a->format == RKV_CACHE_Q8 && a->rule == RKV_Q8_HARSERVE))
     return fail(RKV_ERR_INVALID_ARG, op, "rule=%d", a->rule);
@@ -1387,7 +1399,7 @@ rkv_status rkv_append_rope(rkv_ctx *ctx, const rkv_kv_geometry *g, void *pages, 
     if (rkv_status s = check_rope(a->rope, D, true, op)) return s;
   const bool in16 = a->src_dtype == RKV_BF16;
   const bool with_q = a->q_src != nullptr;
-  if (with_q && (a->q_heads < 1 || !dtype_ok(a->q_out_dtype)))
+  if (with_q && (a->q_heads < 1 || a->q_heads > kMaxHeads || !dtype_ok(a->q_out_dtype)))
     return fail(RKV_ERR_INVALID_ARG, op, "q_heads=%d q_out_dtype=%d", a->q_heads, a->q_out_dtype);
   if (a->n_rows > 0) {
     if (!a->seq_ids || !a->positions) return fail(RKV_ERR_INVALID_ARG, op, "NULL seq_ids/positions");
@@ -1425,8 +1437,8 @@ rkv_status rkv_read_rows(rkv_ctx *ctx, const rkv_kv_geometry *g, int32_t format,
                          int32_t out_dtype, void *stream) {
   const char *op = "rkv_read_rows";
   if (rkv_status s = check_format(g, format, op)) return s;
-  if (rkv_status s = check_tables(pages, block_tables, bt_stride, n_seqs, op)) return s;
-  if (n_rows < 0) return fail(RKV_ERR_INVALID_ARG, op, "n_rows=%d", n_rows);
+  if (rkv_status s = check_whole_words(pages, block_tables, bt_stride, n_seqs, op)) return s;
+  if (n_rows < 0 || n_rows > kMaxRows) return fail(RKV_ERR_INVALID_ARG, op, "n_rows=%d", n_rows);
   if (!dtype_ok(out_dtype)) return fail(RKV_ERR_UNSUPPORTED, op, "out_dtype=%d", out_dtype);
   if (n_rows > 0 && (!seq_ids || !positions)) return fail(RKV_ERR_INVALID_ARG, op, "NULL seq_ids/positions");
   if (reinterpret_cast<uintptr_t>(k_out) % 16 != 0 || reinterpret_cast<uintptr_t>(v_out) % 16 != 0)
@@ -1561,7 +1573,7 @@ rkv_status rkv_decode_mx4(rkv_ctx *ctx, const rkv_kv_geometry *g, const void *pa
   const char *op = "rkv_decode_mx4";
   if (rkv_status s = check_mx4_geometry(g, op)) return s;
   if (rkv_status s = check_decode(g, a, op)) return s;
-  if (rkv_status s = check_tables(pages, block_tables, bt_stride, n_seqs, op)) return s;
+  if (rkv_status s = check_whole_words(pages, block_tables, bt_stride, n_seqs, op)) return s;
   if (!seq_lens) return fail(RKV_ERR_INVALID_ARG, op, "seq_lens is NULL");
   if (a->append)
     return fail(RKV_ERR_UNSUPPORTED, op, "append: 4-bit rows are appended by rkv_append_rope");

@@ -237,3 +237,26 @@ def test_copy_pages(rkv, ctx):
     assert (pages == want).all()
     with pytest.raises(rkv.RkvError, match="stride"):
         rkv.mx4_copy_pages(ctx, g, pages, 5 * n - 16, 2, pairs, 4)
+
+
+def test_host_pool_takes_rotated_rows(rkv, ctx):
+    """Q8_0 pages in host memory: the bytes of the device pool's."""
+    import torch
+    rng = np.random.default_rng(6)
+    rope = rkv.rope_args(D, torch.from_numpy((0.5 ** np.arange(D // 2)).astype(np.float32)).cuda())
+    n = 37
+    x = torch.from_numpy(_rows(rng, n)).cuda()
+    ids = torch.zeros(n, dtype=torch.int32, device="cuda")
+    pos = torch.arange(n, dtype=torch.int32, device="cuda")
+    got = []
+    for memory in (rkv.PAGES_DEVICE, rkv.PAGES_HOST):
+        pool = rkv.Pool(ctx, 1, HKV, D, PT, 8, 1, 4, seed=4, page_memory=memory)
+        pool.alloc.reserve(0, n)
+        pool.sync_tables()
+        pool.append_rope(0, ids, pos, x[:, HQ:HQ + HKV], x[:, HQ + HKV:], rope)
+        k, v = torch.empty(n, HKV, D, device="cuda"), torch.empty(n, HKV, D, device="cuda")
+        pool.read_rows(0, ids, pos, k, v)
+        ctx.sync()
+        got.append((k, v))
+        pool.close()
+    assert (got[0][0] == got[1][0]).all() and (got[0][1] == got[1][1]).all() and (got[0][0] != 0).any()

@@ -164,3 +164,69 @@ def test_rows_are_the_decodes(rkv, ctx):
         c.lens_d = torch.from_numpy(c.lens).cuda()
         one = decode(rkv, ctx, c, q[i][None, None], 1 / 16)
         check(out[i], one[0, 0].cpu().numpy().astype(np.float64), False, f"row {i}")
+
+
+def test_captured_and_replayed(rkv, ctx):
+    """A split chunk captured once and replayed with other queries, eager calls
+    between: every replay bit for bit the eager call's."""
+    import torch
+    entries = [(0, 1500, 30), (1, 10, 20)]
+    c = Cache(rkv, 2, 256, 32, [1530, 30], seed=17)
+    q, _ = query((50, 16, 256), 18, True)
+    out = torch.empty(q.shape, dtype=torch.bfloat16, device="cuda")
+
+    def args(w=None):
+        return rkv.prefill_args([0, 1], [1500, 10], [30, 20], q, out, 0.06, segment_tokens=512, workspace=w)
+    need = rkv.prefill_mx4_workspace_bytes(c.g, args())
+    assert need > 0
+    a = args(torch.full((need,), 255, dtype=torch.uint8, device="cuda"))
+    other = args(torch.full((need,), 255, dtype=torch.uint8, device="cuda"))
+    rkv.prefill_mx4(ctx, c.g, c.pages, c.bt_d, 2, a)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        rkv.prefill_mx4(ctx, c.g, c.pages, c.bt_d, 2, a)
+    for i in range(4):
+        q.copy_(query((50, 16, 256), 30 + i, True)[0])
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        out.zero_()
+        rkv.prefill_mx4(ctx, c.g, c.pages, c.bt_d, 2, other)
+        ctx.sync()
+        assert (out == got).all() and (got != 0).any()
+
+
+def test_pages_behind_32_bits(rkv, ctx):
+    """Pages whose bytes start past 2^32: rows go in, come back, are attended by
+    a decode and a chunk, and pages of the same numbers modulo 2^32 stay."""
+    import torch
+    Hkv, D, PT, Hq, L = 2, 256, 64, 16, 200
+    g1 = rkv.geometry(Hkv, D, PT, 1)
+    n = (1 << 32) // rkv.mx4_page_bytes(g1) + 16
+    g = rkv.geometry(Hkv, D, PT, n)
+    rng = np.random.default_rng(19)
+    pages = torch.empty(n, rkv.mx4_page_bytes(g), dtype=torch.uint8, device="cuda")
+    pages[:40].fill_(9)
+    bt = torch.tensor([[n - 1, n - 7, n - 3, n - 12]], dtype=torch.int32, device="cuda")
+    x = rng.standard_normal((L, 2 * Hkv, D)).astype(np.float32)
+    t = torch.from_numpy(x).cuda()
+    ids = torch.zeros(L, dtype=torch.int32, device="cuda")
+    pos = torch.arange(L, dtype=torch.int32, device="cuda")
+    rkv.append_rope(ctx, g, rkv.CACHE_MX4, pages, bt, ids, pos, t[:, :Hkv], t[:, Hkv:])
+    k, v = torch.empty(L, Hkv, D, device="cuda"), torch.empty(L, Hkv, D, device="cuda")
+    rkv.read_rows(ctx, g, rkv.CACHE_MX4, pages, bt, ids, pos, k, v)
+    ctx.sync()
+    assert (pages[:40] == 9).all()
+    kn, vn = mx4_ref.quantize(x[:, :Hkv], "k")[2], mx4_ref.quantize(x[:, Hkv:], "v")[2]
+    assert (k.cpu().numpy() == kn).all() and (v.cpu().numpy() == vn).all()
+    q, qn = query((30, Hq, D), 20, True)
+    want = mx4_ref.attend(qn, kn, vn, 1 / 16, L - 30 + 1 + np.arange(30))
+    out = torch.empty(q.shape, device="cuda")
+    rkv.prefill_mx4(ctx, g, pages, bt, 1, rkv.prefill_args([0], [L - 30], [30], q, out, 1 / 16))
+    one = torch.empty(1, 1, Hq, D, device="cuda")
+    rkv.decode_mx4(ctx, g, pages, bt, torch.tensor([L], dtype=torch.int32, device="cuda"),
+                   rkv.decode_args(q[29:][None], one, ids[:1], 1 / 16, L))
+    ctx.sync()
+    close(out, want, False, "chunk")
+    close(one[0, 0][None], want[29:], False, "decode")

@@ -134,3 +134,22 @@ def test_binding_refuses_what_it_would_misread(rkv):
             rkv.append_rope(Ctx, g, rkv.CACHE_MX4, bt, bt, sid, pos, k, v, rope, stream=0)
     with pytest.raises(ValueError):
         rkv.read_rows(Ctx, g, rkv.CACHE_MX4, bt, bt, pos, pos, q[:, :, :64], None, stream=0)
+
+
+def test_pages_in_whole_words_and_row_limits(rkv):
+    """Pages off 16 bytes and calls beyond the documented sizes are refused."""
+    g = rkv.geometry(2, 128, 32, 10)
+    rope = _rope(rkv)
+    lib, err = rkv.lib(), lambda: rkv.lib().rkv_last_error().decode()
+    a = rkv.AppendRopeArgs(5, 64, 64, 64, 64, 0, 0, rkv.BF16, rkv.CACHE_MX4, 0, C.pointer(rope), 64, 0, 8, 64, rkv.BF16)
+    assert lib.rkv_append_rope(None, C.byref(g), 72, 64, 4, 2, C.byref(a), None) == -1 and "pages" in err()
+    assert lib.rkv_read_rows(None, C.byref(g), 1, 72, 64, 4, 2, 3, 64, 64, 64, 64, 0, None) == -1 and "pages" in err()
+    assert lib.rkv_read_rows(None, C.byref(g), 1, 64, 64, 4, 2, (1 << 23) + 1, 64, 64, 64, 64, 0, None) == -1
+    assert "n_rows" in err()
+    for over in ({"n_rows": (1 << 23) + 1}, {"q_heads": 1 << 15}):
+        assert _append(rkv, g, **over)[0] == -1
+        assert _rows(rkv, rope, **over)[0] == -1
+    d = rkv.DecodeArgs(2, 64, 64, rkv.BF16, 1, 8, 0.1, 64, rkv.F32, 0, 4096, 64, 0, None, None)
+    assert lib.rkv_decode_mx4(None, C.byref(g), 72, 64, 8, 64, 2, C.byref(d), None) == -1 and "pages" in err()
+    p = rkv.PrefillArgs()
+    assert lib.rkv_prefill_mx4(None, C.byref(g), 72, 64, 8, 2, C.byref(p), None) == -1 and "pages" in err()

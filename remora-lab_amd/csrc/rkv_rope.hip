@@ -181,14 +181,25 @@ __device__ __forceinline__ void store4(void *out, int64_t at, bool bf16, const f
     *reinterpret_cast<v4f *>(static_cast<float *>(out) + at) = v4f{v[from], v[from + 1], v[from + 2], v[from + 3]};
 }
 
-// A norm weight's values at a lane's dims.
+// A norm weight's values at a lane's dims, 4 at a time (a choice for each
+// value would wait for eight loads one after the other).  A weight lies where
+// its own type may.
+typedef uint32_t v2u_any __attribute__((ext_vector_type(2), aligned(2)));
+typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
 __device__ __forceinline__ void load_weight(const void *w, bool bf16, const Dims &d, float (&v)[8]) {
+  if (w == nullptr) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int at = i < 4 ? d.a + i : d.b + i - 4;
-    v[i] = w == nullptr ? 1.0f
-           : bf16       ? bf16_bits_to_f32(static_cast<const uint16_t *>(w)[at])
-                        : static_cast<const float *>(w)[at];
+    for (int i = 0; i < 8; ++i) v[i] = 1.0f;
+  } else if (bf16) {
+    const uint16_t *p = static_cast<const uint16_t *>(w);
+    const v2u_any x[2] = {*reinterpret_cast<const v2u_any *>(p + d.a), *reinterpret_cast<const v2u_any *>(p + d.b)};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = bf16_bits_to_f32((uint16_t)(x[i / 4][i % 4 / 2] >> (16 * (i & 1))));
+  } else {
+    const float *p = static_cast<const float *>(w);
+    const v4f_any x[2] = {*reinterpret_cast<const v4f_any *>(p + d.a), *reinterpret_cast<const v4f_any *>(p + d.b)};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = x[i / 4][i % 4];
   }
 }
 
@@ -231,8 +242,25 @@ struct HeadRange {
   int h0, h1;
 };
 
-// Heads of one row, by one wave, 512/D at a time in batches of kBatch loads:
-// those of `one`, then those of `two`; the first batch is on its way while the
+// A lane's 8 values of a head as they lie in memory.
+template <bool kBf16>
+struct HeadValues {
+  using Half = typename std::conditional<kBf16, v2u, v4f>::type;
+  Half w[2];
+  __device__ __forceinline__ void load(const void *src, int64_t at, const Dims &d) {
+    using T = typename std::conditional<kBf16, uint16_t, float>::type;
+    const T *p = static_cast<const T *>(src) + at;
+    w[0] = *reinterpret_cast<const Half *>(p + d.a);
+    w[1] = *reinterpret_cast<const Half *>(p + d.b);
+  }
+  __device__ __forceinline__ float operator[](int i) const {
+    if constexpr (!kBf16) return w[i / 4][i % 4];
+    else return __builtin_bit_cast(float, i & 1 ? w[i / 4][i % 4 / 2] & 0xffff0000u : w[i / 4][i % 4 / 2] << 16);
+  }
+};
+
+// Heads of one row, by one wave, 512/D at a time: those of `one`, then those
+// of `two`, kAhead steps of loads on their way.  The first go out before the
 // row's cosines are computed, a pair or two a lane, and passed round through
 // `turns` (the wave's own).  A pair's values, weights, cosine and sine meet in
 // four products that are the row's, so a head costs two products a value and
@@ -240,100 +268,91 @@ struct HeadRange {
 template <int D, bool kIn16, bool kOut16, bool kAdjacent>
 __device__ __forceinline__ void turn_row(const RopeLaunch &r, const HeadRange &one, const HeadRange &two, int64_t row,
                                          int32_t pos, int lane, float2 (&turns)[D / 2]) {
-  constexpr int L = D / 8, kHeads = 64 / L, kBatch = 4;
+  constexpr int L = D / 8, kHeads = 64 / L, kAhead = 4;
   const int c = lane % L;
   const Dims d(r, c);
   const bool rotated = 8 * c < r.rot_dim;
-  float tc[4], ts[4];
-  bool turn = true;
-#pragma unroll 1
-  for (int kind = one.h0 < one.h1 ? 0 : 1; kind < 2; ++kind) {
-    const HeadRange &g = kind == 0 ? one : two;
-    if (g.h0 >= g.h1) break;
-    const bool norm = g.weight != nullptr;
-    const int64_t src = row * g.m.stride, dst = row * g.m.out_stride;
-    float v[kBatch][8];
-    auto load = [&](int first) {
+  const int n1 = (max(one.h1 - one.h0, 0) + kHeads - 1) / kHeads;
+  const int n = n1 + (max(two.h1 - two.h0, 0) + kHeads - 1) / kHeads;
+  if (n == 0) return;
+  HeadValues<kIn16> v[kAhead];
+  auto head = [&](int i) { return (i < n1 ? one.h0 + i * kHeads : two.h0 + (i - n1) * kHeads) + lane / L; };
+  auto load = [&](int i) {
+    const int h = min(head(i), (i < n1 ? one.h1 : two.h1) - 1);
+    v[i % kAhead].load(i < n1 ? one.m.src : two.m.src, row * (i < n1 ? one.m.stride : two.m.stride) + (int64_t)h * D, d);
+  };
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        if (first + k * kHeads >= g.h1) break;
-        const int h = min(first + k * kHeads + lane / L, g.h1 - 1);
-        load4(g.m.src, src + (int64_t)h * D + d.a, kIn16, v[k], 0);
-        load4(g.m.src, src + (int64_t)h * D + d.b, kIn16, v[k], 4);
-      }
-    };
-    load(g.h0);
-    float w[8];
-    load_weight(g.weight, r.norm_bf16 != 0, d, w);
-    if (turn) {
-      int32_t at[4] = {pos, pos, pos, pos};
-      if (r.positions != nullptr)
+  for (int i = 0; i < kAhead; ++i)
+    if (i < n) load(i);
+  float w[2][8];
+  load_weight(one.weight, r.norm_bf16 != 0, d, w[0]);
+  load_weight(two.weight, r.norm_bf16 != 0, d, w[1]);
+  int32_t at[4] = {pos, pos, pos, pos};
+  if (r.positions != nullptr)
 #pragma unroll
-        for (int a = 0; a < 4; ++a) at[a] = r.positions[(int64_t)min(a, r.n_axes - 1) * r.n_rows + row];
+    for (int a = 0; a < 4; ++a) at[a] = r.positions[(int64_t)min(a, r.n_axes - 1) * r.n_rows + row];
 #pragma unroll
-      for (int pair = lane; pair < D / 2; pair += 64) {
-        if (2 * pair >= r.rot_dim) break;
-        double s, co;
-        sin_cos(angle(r, pair, at), s, co);
-        turns[pair] = float2{(float)co, (float)s};
-      }
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 u = rotated ? turns[4 * c + i] : float2{1.0f, 0.0f};
-        tc[i] = u.x;
-        ts[i] = u.y;
-      }
-      turn = false;
-    }
-    // y[a] = x[a] * ca + x[b] * -sb, y[b] = x[b] * cb + x[a] * sa
-    float ca[4], cb[4], sa[4], sb[4];
+  for (int pair = lane; pair < D / 2; pair += 64) {
+    if (2 * pair >= r.rot_dim) break;
+    double si, co;
+    sin_cos(angle(r, pair, at), si, co);
+    turns[pair] = float2{(float)co, (float)si};
+  }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  // y[a] = x[a] * ca + x[b] * -sb, y[b] = x[b] * cb + x[a] * sa
+  float ca[4], cb[4], sa[4], sb[4];
+  auto weigh = [&](const float (&x)[8]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float wa = w[kAdjacent ? 2 * i : i], wb = w[kAdjacent ? 2 * i + 1 : i + 4];
-      ca[i] = tc[i] * wa;
-      cb[i] = tc[i] * wb;
-      sa[i] = ts[i] * wa;
-      sb[i] = ts[i] * wb;
+      const float wa = x[kAdjacent ? 2 * i : i], wb = x[kAdjacent ? 2 * i + 1 : i + 4];
+      const float2 u = rotated ? turns[4 * c + i] : float2{1.0f, 0.0f};
+      ca[i] = u.x * wa;
+      cb[i] = u.x * wb;
+      sa[i] = u.y * wa;
+      sb[i] = u.y * wb;
     }
-    for (int first = g.h0;;) {
+  };
+  weigh(w[0]);
+  for (int base = 0; base < n; base += kAhead)
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        if (first + k * kHeads >= g.h1) break;
-        const int h = first + k * kHeads + lane / L;
-        float f = 1.0f;
-        if (norm) {
-          float q = v[k][0] * v[k][0];
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = base + k;
+      if (i >= n) break;
+      if (i == n1) weigh(w[1]);
+      const HeadValues<kIn16> &x = v[k];
+      const bool norm = (i < n1 ? one.weight : two.weight) != nullptr;
+      float f = 1.0f;
+      if (norm) {
+        float q = x[0] * x[0];
 #pragma unroll
-          for (int i = 1; i < 8; ++i) q = __builtin_fmaf(v[k][i], v[k][i], q);
-          f = inv_sqrt(lanes_sum<L>(q) * (1.0f / D) + r.eps);
-        }
-        float y[8];
+        for (int e = 1; e < 8; ++e) q = __builtin_fmaf(x[e], x[e], q);
+        f = inv_sqrt(lanes_sum<L>(q) * (1.0f / D) + r.eps);
+      }
+      float y[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int a = kAdjacent ? 2 * i : i, b = kAdjacent ? 2 * i + 1 : i + 4;
-          y[a] = v[k][a] * ca[i];
-          y[b] = v[k][b] * cb[i];
-          if (rotated) {  // (not a sine of 0: it would make NaN of an infinite partner)
-            y[a] = __builtin_fmaf(v[k][b], -sb[i], y[a]);
-            y[b] = __builtin_fmaf(v[k][a], sa[i], y[b]);
-          }
-        }
-        if (norm) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] *= f;
-        }
-        if (h < g.h1) {
-          store4(g.m.out, dst + (int64_t)h * D + d.a, kOut16, y, 0);
-          store4(g.m.out, dst + (int64_t)h * D + d.b, kOut16, y, 4);
+      for (int e = 0; e < 4; ++e) {
+        const int a = kAdjacent ? 2 * e : e, b = kAdjacent ? 2 * e + 1 : e + 4;
+        y[a] = x[a] * ca[e];
+        y[b] = x[b] * cb[e];
+        if (rotated) {  // (not a sine of 0: it would make NaN of an infinite partner)
+          y[a] = __builtin_fmaf(x[b], -sb[e], y[a]);
+          y[b] = __builtin_fmaf(x[a], sa[e], y[b]);
         }
       }
-      first += kBatch * kHeads;
-      if (first >= g.h1) break;
-      load(first);
+      if (norm) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] *= f;
+      }
+      if (i + kAhead < n) load(i + kAhead);
+      const int h = head(i);
+      if (h < (i < n1 ? one.h1 : two.h1)) {
+        void *out = i < n1 ? one.m.out : two.m.out;
+        const int64_t to = row * (i < n1 ? one.m.out_stride : two.m.out_stride) + (int64_t)h * D;
+        store4(out, to + d.a, kOut16, y, 0);
+        store4(out, to + d.b, kOut16, y, 4);
+      }
     }
-  }
 }
 
 template <int D, bool kIn16, bool kOut16>

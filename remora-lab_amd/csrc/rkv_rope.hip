@@ -9,7 +9,7 @@
 // Angles are exact in f64 (24 + 31 bits) and reduced there, so a position of a
 // million keeps every bit.  A key on its way into the cache is normed and
 // rotated in f64 and rounded to f32 once, before the quantizer: f64 runs at
-// the f32 rate here, and a page byte then follows from the definition alone,
+// half the f32 rate here, and a page byte then follows from the definition alone,
 // not from an order of sums (an f32 rotation moves about one code in 10^6 over
 // a border).  Rows that are returned go in f32.
 //
@@ -363,7 +363,9 @@ __device__ __forceinline__ void turn_row(const RopeLaunch &r, const HeadRange &o
 }
 #endif  // __HIP_DEVICE_COMPILE__
 
-// Four rows a workgroup, a row a wave; blockIdx.y: which `chunk` of the row's
+// Bound by memory from about 8000 rows on: 32,768 rows of 18 heads of 128 bf16
+// values 52.5 us, 5.8 TB/s read and written; 4099 rows 8.9 us, 4.2 TB/s; a
+// single row is a launch.  Four rows a workgroup, a row a wave; blockIdx.y: which `chunk` of the row's
 // query heads and then key heads, counted through.
 template <int D, bool kIn16, bool kOut16>
 __global__ __launch_bounds__(256) void rope_rows_kernel(RopeLaunch r, HeadRows q, HeadRows k, int32_t chunk) {
@@ -381,8 +383,9 @@ __global__ __launch_bounds__(256) void rope_rows_kernel(RopeLaunch r, HeadRows q
 
 // ---- append ------------------------------------------------------------------------
 // kv heads of a workgroup, which share a row's cosines: two of a large call's
-// rows (65,619 rows of 2 heads 82.6 -> 62 us), one of a small call's, where
-// the second would wait for the first (64 rows 9.1 -> 12.8 us a call).
+// rows (65,619 rows of 2 heads into 4-bit pages 82 -> 74 us without queries, 38
+// unrotated), one of a small call's, where the second would wait for the first
+// (64 rows 9.1 -> 12.8 us a call).
 constexpr int append_heads(int rows) { return rows == 32 ? 2 : 1; }
 
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -422,9 +425,9 @@ __device__ __forceinline__ uint32_t low_nibbles(uint32_t w0, uint32_t w1) {
 }
 #endif  // __HIP_DEVICE_COMPILE__
 
-// Workgroup x of the first append_blocks takes input rows [ROWS*(x / groups),
-// +ROWS) and kv heads [kHeads*(x % groups), +kHeads); the others are the query
-// waves (rope_rows_kernel's, keys none).
+// Workgroup x = i * every, i < append_blocks, takes input rows [ROWS*(i /
+// groups), +ROWS) and kv heads [kHeads*(i % groups), +kHeads); the others are
+// the query waves (rope_rows_kernel's, keys none).
 //  1. wave 0 finds each row's page and slot; rows that have none are reported
 //     and skipped.
 //  2. 512/D rows a wave: K normed and rotated in f64, through LDS into 8
@@ -437,9 +440,13 @@ __device__ __forceinline__ uint32_t low_nibbles(uint32_t w0, uint32_t w1) {
 //     whole words, 16 bytes a lane.  A run that does not fill its group leaves
 //     the other tokens' bits alone: bytes, and in 4-bit pages an atomic xor of
 //     the V words' own bits (another run of the call may hold the rest).
+// Bound by memory but for the f64 of the rotation: 65,619 rows of 16 query and
+// 2 kv heads of 256 bf16 values into 4-bit pages 232 us, 5.3 TB/s read and
+// written; their keys and values alone 75 us, 39 unrotated.  4096 rows into
+// Q8_0 pages 21 us, 64 rows 9 us (latency: page ids, rows, runs).
 template <int D, bool kMx4, int ROWS, bool kBf16>
 __global__ __launch_bounds__(256) void append_rope_kernel(AppendRopeLaunch p, int32_t groups, uint32_t append_blocks,
-                                                          int32_t chunk) {
+                                                          uint32_t every, int32_t chunk) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int L = D / 8, RW = 64 / L, NB = D / 32, H = D / 128;
   constexpr int GROUP = kMx4 ? 8 : 4;        // tokens of a V word
@@ -458,8 +465,9 @@ __global__ __launch_bounds__(256) void append_rope_kernel(AppendRopeLaunch p, in
   const Geo g = a.g;
   const int tid = (int)threadIdx.x, lane = tid & 63;
   const int wave = (int)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (blockIdx.x >= append_blocks) {
-    const uint32_t nq = (uint32_t)(p.q.heads + chunk - 1) / (uint32_t)chunk, x = blockIdx.x - append_blocks;
+  const uint32_t nth = blockIdx.x / every;
+  if (nth >= append_blocks || blockIdx.x % every != 0) {
+    const uint32_t nq = (uint32_t)(p.q.heads + chunk - 1) / (uint32_t)chunk, x = blockIdx.x - min(nth + 1, append_blocks);
     const int64_t row = (int64_t)(x / nq) * 4 + wave;
     const int at = (int)(x % nq) * chunk;
     if (row < a.n_rows)
@@ -468,8 +476,8 @@ __global__ __launch_bounds__(256) void append_rope_kernel(AppendRopeLaunch p, in
                                 *reinterpret_cast<float2(*)[D / 2]>(&turned[wave][0][0]));
     return;
   }
-  const int64_t row0 = (int64_t)(blockIdx.x / groups) * ROWS;
-  const int h0 = (int)(blockIdx.x % groups) * kHeads, nh = min(g.kv_heads - h0, kHeads);
+  const int64_t row0 = (int64_t)(nth / groups) * ROWS;
+  const int h0 = (int)(nth % groups) * kHeads, nh = min(g.kv_heads - h0, kHeads);
   const int nr = (int)min<int64_t>(ROWS, (int64_t)a.n_rows - row0);
   const uint64_t PB = kMx4 ? mx4_page_bytes(g) : page_bytes(g);
   const uint64_t RB = kMx4 ? mx4_region_bytes(g) : region_bytes(g);
@@ -662,7 +670,10 @@ __global__ __launch_bounds__(256) void append_rope_kernel(AppendRopeLaunch p, in
 
 // ---- rows read back -----------------------------------------------------------------
 
-// One thread per 8 consecutive dims of a row; blockIdx.y: (kv head, kind).
+// One thread per 8 consecutive dims of a row; blockIdx.y: (kv head, kind).  A
+// V row's values lie 8 (Q8_0: 32) tokens apart, so rows that follow each other
+// share their lines in the L1.  65,619 rows of 4-bit pages into bf16 50 us (170
+// MB in all), 4096 of Q8_0 9.5 us.
 template <int D, bool kMx4>
 __global__ __launch_bounds__(256) void read_rows_kernel(ReadRowsLaunch p) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -737,8 +748,9 @@ __global__ __launch_bounds__(256) void read_rows_kernel(ReadRowsLaunch p) {
 #endif  // __HIP_DEVICE_COMPILE__
 }
 
-// Heads of a query wave: a row's heads over so many waves that the launch has
-// about 4096 (16 a CU), each wave's cosines serving all of its heads.
+// Heads of a wave: a row's heads over so many waves that the launch has about
+// 4096 (16 a CU), as each computes its row's cosines for all of them (2048 or
+// 8192 waves: the same within 0.6 us from 1024 to 32,768 rows of 18 heads).
 int32_t head_chunk(int64_t rows, int32_t heads, int32_t per) {
   const int64_t want = std::max<int64_t>(1, (int64_t)heads * rows / 4096);
   return (int32_t)std::min<int64_t>((want + per - 1) / per * per, (heads + per - 1) / per * per);
@@ -751,25 +763,28 @@ void launch_append_rope_r(const AppendRopeLaunch &p, hipStream_t s) {
   const uint32_t blocks = (uint32_t)(row_blocks * groups);
   uint32_t q_blocks = 0;
   int32_t chunk = 1;
-  if (ROWS == 8 && p.q.src != nullptr && p.q.bf16 == p.q.out_bf16) {
+  if (p.q.src != nullptr && p.q.bf16 == p.q.out_bf16) {
     chunk = head_chunk(p.a.n_rows, p.q.heads, 512 / D);
     q_blocks = (uint32_t)((p.a.n_rows + 3LL) / 4 * ((p.q.heads + chunk - 1) / chunk));
   }
+  // A small call's append goes first, a large one's is spread over the launch:
+  // its f64 then runs beside the queries' loads (65,619 rows in one launch 232
+  // us, in two 256; an odd step, as every 8th workgroup is on one XCD: 449).
+  uint32_t every = ROWS == 8 ? 1 : (blocks + q_blocks) / blocks;
+  every -= every % 2 == 0;
   if (p.a.src_bf16)
     hipLaunchKernelGGL((append_rope_kernel<D, kMx4, ROWS, true>), dim3(blocks + q_blocks), dim3(256), 0, s, p, groups,
-                       blocks, chunk);
+                       blocks, every, chunk);
   else
     hipLaunchKernelGGL((append_rope_kernel<D, kMx4, ROWS, false>), dim3(blocks + q_blocks), dim3(256), 0, s, p, groups,
-                       blocks, chunk);
+                       blocks, every, chunk);
 }
-// 32-row workgroups once there are at least 8 per CU, else 8-row ones, which
-// take the queries into the launch: a large call's go by themselves, since the
-// append's registers leave a CU half as many of their waves (and so do those
-// of another type than the rows').
+// 32-row workgroups once there are at least 8 per CU, else 8-row ones.
 bool small_call(const AppendRopeLaunch &p) {
   return (int64_t)p.a.n_rows * p.a.g.kv_heads < (int64_t)32 * 8 * kComputeUnits;
 }
-bool queries_with(const AppendRopeLaunch &p) { return small_call(p) && p.q.bf16 == p.q.out_bf16; }
+// Queries of another type than the rows' go by themselves.
+bool queries_with(const AppendRopeLaunch &p) { return p.q.bf16 == p.q.out_bf16; }
 template <int D, bool kMx4>
 void launch_append_rope_d(const AppendRopeLaunch &p, hipStream_t s) {
   if (small_call(p)) launch_append_rope_r<D, kMx4, 8>(p, s);

@@ -264,9 +264,9 @@ struct Mx4Rows {
 };
 
 // G groups of rows that share the widened K and V of a tile.
-template <int D, int G, bool kTwo, bool kBf16>
-struct Mx4Wide : Mx4Rows<D, G, kTwo> {
-  using Rows = Mx4Rows<D, G, kTwo>;
+template <int D, int G, bool kBf16>
+struct Mx4Wide : Mx4Rows<D, G, true> {
+  using Rows = Mx4Rows<D, G, true>;
   using Rows::acc, Rows::rlim, Rows::lane, Rows::lg;
   static constexpr int H = D / 128, NB = D / 32;
   using Query = Mx4Query<D, false, kBf16>;

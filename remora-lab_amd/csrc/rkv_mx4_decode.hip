@@ -26,8 +26,17 @@
 //   f16 range: M is kept so that p * 2^e_v <= 2^15, i.e. with vcap the largest V
 //   exponent met (at least 2^0 in the units of the stored byte) the row maximum
 //   maps to 2^(11 - vcap) and may rise by 2^4 before the sums are rescaled.
-// 9 to 32 rows (Mx4Wide, which the prefill shares): one or two groups of 16
-// columns, V widened with its scales once for all of them, the query in LDS.
+// 9 to 32 rows (Mx4Wide): one or two groups of 16 columns, V widened with its
+// scales once for all of them, the query in LDS.
+//
+// Measured (2 kv heads of 256, bf16 queries): 64 x 32k tokens of 8 rows 180 us
+// a call, 6.4 TB/s (a read of the same pages in the same order 165); one
+// sequence of 262,145 tokens 35 us, 16 of 4k..16k 26, one of 300 8: locating
+// the partition, its page ids and its first tile come one after the other, and
+// a second launch joins partials (4.5 us).  32 x 32k tokens of 32 rows 131 us
+// (memory alone 83): 2 waves a SIMD issue 290 vector and 96 matrix instructions
+// a tile.  Not faster: two tiles in flight, a third wave a SIMD, 8 waves a
+// workgroup.
 #include <algorithm>
 
 #include "rkv_mx4_attn.h"
@@ -311,7 +320,7 @@ __global__ __launch_bounds__(64 * NW, kMx4WgsPerCu) void mx4_decode_kernel(Decod
 template <int D, int G, bool kBf16, int NW>
 __global__ __launch_bounds__(64 * NW, kMx4WgsPerCu) void mx4_decode_wide_kernel(DecodeLaunch p) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  using Dec = Mx4Wide<D, G, true, kBf16>;  // (weights of two terms cost a verify of 32 x 32k rows 1 us of 152)
+  using Dec = Mx4Wide<D, G, kBf16>;  // (weights of two terms cost a verify of 32 x 32k rows 1 us of 152)
   constexpr int kStride = D + 4;
   constexpr int kShared = Dec::kQuery * 16 > 16 * G * kStride * 4 ? Dec::kQuery * 16 : 16 * G * kStride * 4;
   __shared__ __attribute__((aligned(16))) uint8_t shared[kShared];

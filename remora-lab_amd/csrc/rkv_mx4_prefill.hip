@@ -1,21 +1,32 @@
 // rkv_mx4_prefill.hip -- chunked prefill attention over 4-bit pages (rkv_mx4.h)
-// for gfx950: the units, causal ranges, split plan and combine of
-// rkv_prefill.hip with a kernel of its own.
+// for gfx950: the units, causal ranges and combine of rkv_prefill.hip with a
+// kernel of its own.
 //
 // A workgroup of 4 waves takes a block of 128 query rows of one (entry, kv
-// head), wave w rows 32w .. 32w+31 as two column groups of 16.  The waves
-// share nothing: each walks the block's tiles by itself, up to the last
-// position that its own rows attend, and loads them straight into registers
-// (the other waves' loads of the same tile come from the CU's L1 or the L2).
-//   QK: bf16 16x16x32 on K codes widened with their scales, exact.
+// head), wave w rows 32w .. 32w+31 as two column groups of 16, and walks the
+// block's tiles of 32 tokens.
+//   QK: bf16 16x16x32 on K codes widened with their scales, exact.  Each wave
+//     loads the tile's K codes (the CU's L1 serves four of them) and widens
+//     them itself.
 //   PV: f16 16x16x32 on V codes times their scales, exact in f16 too, and held
 //     times 2^6: 2^-17 to 6 * 2^13 (the product of a subnormal f16 keeps the
 //     bits that its unnormalised exponent leaves: without the 2^6 V of 3e-7
 //     came out 1.3e-5 off).  One product of the weights cut to f16 for bf16
 //     rows (11 bits: 1.4e-4 of a row beside the 1.7e-3 of its own rounding),
-//     two for f32 rows (22 bits).
-// The scales cost a multiplication per widened V value and none per weight:
-// 64 packed products a tile for all 32 rows at head_dim 256.
+//     two for f32 rows (22 bits).  V costs a conversion and a multiplication a
+//     pair, so each wave widens a quarter of the next tile's into LDS, in two
+//     buffers, one barrier a tile.
+// Bound by issue: besides a 16-cycle matrix instruction a SIMD issues about two
+// others, from either of its two waves, and each further one costs 4.6 cycles.
+// A wave's tile takes 96 matrix instructions for f32 rows (64 for bf16) and 180
+// others at head_dim 256; widening V in every wave took 303 (804 us for the
+// first case below).  The queries' first half stays in registers and the second
+// in LDS: both in LDS leave no room for two workgroups a CU, both in registers
+// spill.
+// Measured (2 kv heads of 256, 8 query heads each): eight chunks of 512 rows
+// after 8192 tokens 694 us with f32 rows (817 TFLOP/s), 552 with bf16 rows
+// (1028); six chunks of 17..701 rows of 24 heads after up to 3000 tokens 150.
+// Not faster: 64 rows a wave, one wave a SIMD (979).
 #include <algorithm>
 #include <type_traits>
 

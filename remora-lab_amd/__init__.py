@@ -673,12 +673,20 @@ def _raw_stream(ctx: Ctx, s):
     return s if isinstance(s, int) else s.cuda_stream
 
 
-def _i32(t, what: str) -> int | None:
-    """Address of a contiguous int32 tensor (or None)."""
+def _i32(t, what: str, device: int | None = None) -> int | None:
+    """Address of a contiguous int32 tensor (or None), on `device` if one is given."""
     if t is None:
         return None
     if t.dtype is not (_torch or _load_torch()).int32 or not t.is_contiguous():
         raise TypeError(f"{what}: a contiguous int32 tensor wanted")
+    if device is not None and t.get_device() != device:
+        raise ValueError(f"{what}: a tensor of device {device} wanted")
+    return t.data_ptr()
+
+
+def _pages(t, device: int) -> int:
+    if t.get_device() != device:
+        raise ValueError(f"pages: a tensor of device {device} wanted")
     return t.data_ptr()
 
 
@@ -691,6 +699,8 @@ def _heads(t, n: int, D: int, dtype, what: str, device: int) -> tuple[int, int, 
         raise ValueError(f"{what}: [{n}][heads][{D}] of {dtype} wanted, got {tuple(t.shape)} of {t.dtype}")
     if s2 != 1 or (h > 1 and s1 != D):
         raise ValueError(f"{what}: dense heads wanted, got strides {t.stride()}")
+    if n > 1 and s0 < h * D:  # (rows over each other; 0 would read as dense)
+        raise ValueError(f"{what}: rows that follow each other wanted, got strides {t.stride()}")
     if t.get_device() != device:
         raise ValueError(f"{what}: a tensor of device {device} wanted")
     return t.data_ptr(), h, s0 if n > 1 else h * D
@@ -716,10 +726,13 @@ def rope_args(rot_dim: int, freqs, positions=None, pair_axis=None, adjacent: boo
     a._refs = (freqs, positions, pair_axis, q_norm, k_norm)
     a._rows = None if positions is None else positions.shape[-1]
     a._dims = [None if w is None else w.numel() for w in (q_norm, k_norm)]
+    a._devices = {t.get_device() for t in a._refs if t is not None}
     return a
 
 
-def _rope_fits(rope: RopeArgs, n: int, D: int) -> None:
+def _rope_fits(rope: RopeArgs, n: int, D: int, device: int) -> None:
+    if not rope._devices <= {device}:
+        raise ValueError(f"rope: tensors of device {device} wanted, got {sorted(rope._devices)}")
     if rope._rows is not None and rope._rows != n:
         raise ValueError(f"{rope._rows} rope positions for {n} rows")
     if rope._dims[0] not in (None, D) or rope._dims[1] not in (None, D):
@@ -732,7 +745,7 @@ def rope_rows(ctx: Ctx, rope: RopeArgs, q, k, q_out, k_out, stream=None) -> None
     one, out = (q, q_out) if q is not None else (k, k_out)
     n, _, D = one.shape
     dtype, otype, dev = one.dtype, out.dtype, ctx.device
-    _rope_fits(rope, n, D)
+    _rope_fits(rope, n, D, dev)
     qp, qh, qs, qo, qos = None, 0, 0, None, 0
     kp, kh, ks, ko, kos = None, 0, 0, None, 0
     if q is not None:
@@ -756,7 +769,7 @@ def append_rope(ctx: Ctx, g: Geometry, fmt: int, pages, block_tables, seq_ids, p
     on the way (rope); q [n][q_heads][head_dim] goes normed and rotated to q_out
     (contiguous)."""
     a = _append_args(ctx, g, fmt, seq_ids, positions, k_src, v_src, rope, q, q_out, rule)
-    check(lib().rkv_append_rope(ctx.h, C.byref(g), pages.data_ptr(), _i32(block_tables, "block_tables"),
+    check(lib().rkv_append_rope(ctx.h, C.byref(g), _pages(pages, ctx.device), _i32(block_tables, "block_tables", ctx.device),
                                 block_tables.shape[-1], block_tables.shape[0], C.byref(a),
                                 _raw_stream(ctx, stream)))
 
@@ -768,7 +781,7 @@ def _append_args(ctx, g, fmt, seq_ids, positions, k_src, v_src, rope, q, q_out, 
     if kh != g.kv_heads or vh != kh or positions.numel() != n:
         raise ValueError("k and v rows have the geometry's heads, and a position each")
     if rope is not None:
-        _rope_fits(rope, n, D)
+        _rope_fits(rope, n, D, dev)
     qp, qh, qs, qo, ot = None, 0, 0, None, F32
     if q is not None:
         qp, qh, qs = _heads(q, n, D, dtype, "q", dev)
@@ -776,7 +789,7 @@ def _append_args(ctx, g, fmt, seq_ids, positions, k_src, v_src, rope, q, q_out, 
         if h != qh or s != h * D:
             raise ValueError("q_out: contiguous, shaped like q")
         ot = _type(q_out.dtype)
-    return AppendRopeArgs(n, _i32(seq_ids, "seq_ids"), _i32(positions, "positions"), kp, vp, ks, vs,
+    return AppendRopeArgs(n, _i32(seq_ids, "seq_ids", dev), _i32(positions, "positions", dev), kp, vp, ks, vs,
                           _type(dtype), fmt, rule, C.pointer(rope) if rope is not None else None, qp, qs, qh, qo, ot)
 
 
@@ -784,7 +797,7 @@ def read_rows(ctx: Ctx, g: Geometry, fmt: int, pages, block_tables, seq_ids, pos
               stream=None) -> None:
     """Values of cached rows into k_out, v_out [n][kv_heads][head_dim] (either may be None)."""
     rows = _read_args(ctx, g, seq_ids, positions, k_out, v_out)
-    check(lib().rkv_read_rows(ctx.h, C.byref(g), fmt, pages.data_ptr(), _i32(block_tables, "block_tables"),
+    check(lib().rkv_read_rows(ctx.h, C.byref(g), fmt, _pages(pages, ctx.device), _i32(block_tables, "block_tables", ctx.device),
                               block_tables.shape[-1], block_tables.shape[0], *rows, _raw_stream(ctx, stream)))
 
 
@@ -802,7 +815,7 @@ def _read_args(ctx, g, seq_ids, positions, k_out, v_out) -> tuple:
         if h != kv or s != kv * D:
             raise ValueError("outputs: contiguous [rows][kv_heads][head_dim]")
         at.append(p)
-    return (n, _i32(seq_ids, "seq_ids"), _i32(positions, "positions"), *at,
+    return (n, _i32(seq_ids, "seq_ids", dev), _i32(positions, "positions", dev), *at,
             _type(out.dtype) if out is not None else F32)
 
 

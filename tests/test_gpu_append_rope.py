@@ -301,3 +301,38 @@ def test_together_and_captured(rkv, ctx):
             assert np.abs(got[s] - want).max() < 2e-5
             turned = mx4_ref.rope(h[-1:, :Hq], fn, p[:, -1:], axis, False, wn, 1e-6)
             assert np.abs(qn - turned).max() <= 2.0 ** -8 * np.abs(turned).max()
+
+
+@pytest.mark.parametrize("n", [3, 33003])
+@pytest.mark.parametrize("src,out", [("float32", "bfloat16"), ("bfloat16", "float32"), ("bfloat16", "bfloat16")])
+def test_queries_are_rope_rows(rkv, ctx, n, src, out):
+    """The append's queries bit for bit rkv_rope_rows', in one launch with the
+    rows or by themselves; a large call's cached rows those of its parts."""
+    import torch
+    Hq, Hkv, D, PT, S = 5, 2, 128, 64, 7
+    src, out = getattr(torch, src), getattr(torch, out)
+    torch.manual_seed(n)
+    x = torch.randn(n, Hq + 2 * Hkv, D, device="cuda").to(src)
+    ids = (torch.arange(n, device="cuda") % S).sort().values.to(torch.int32)
+    pos = torch.cat([torch.arange(int((ids == s).sum()), device="cuda") for s in range(S)]).to(torch.int32)
+    f = torch.from_numpy((100.0 ** (-np.arange(32) / 32)).astype(np.float32)).cuda()
+    w = torch.rand(D, device="cuda") + 0.5
+    W = -(-(n // S + 1) // PT)
+    g = rkv.geometry(Hkv, D, PT, S * W)
+    bt = torch.randperm(S * W, device="cuda").to(torch.int32).view(S, W)
+    q, k, v = x[:, :Hq], x[:, Hq:Hq + Hkv], x[:, Hq + Hkv:]
+    got = []
+    for parts in (1, 3):
+        pages = torch.zeros(S * W * rkv.mx4_page_bytes(g), dtype=torch.uint8, device="cuda")
+        q_out = torch.empty(n, Hq, D, dtype=out, device="cuda")
+        cut = [n * i // parts for i in range(parts + 1)]
+        for a, b in zip(cut, cut[1:]):
+            rope = rkv.rope_args(64, f, pos[a:b], q_norm=w, k_norm=w, eps=1e-6)
+            rkv.append_rope(ctx, g, rkv.CACHE_MX4, pages, bt, ids[a:b], pos[a:b], k[a:b], v[a:b], rope, q[a:b],
+                            q_out[a:b])
+        got.append((pages, q_out))
+    want = torch.empty(n, Hq, D, dtype=out, device="cuda")
+    rkv.rope_rows(ctx, rkv.rope_args(64, f, pos, q_norm=w, k_norm=w, eps=1e-6), q, None, want, None)
+    ctx.sync()
+    assert (got[0][1] == want).all() and (got[1][1] == want).all()
+    assert (got[0][0] == got[1][0]).all()

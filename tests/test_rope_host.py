@@ -153,3 +153,38 @@ def test_pages_in_whole_words_and_row_limits(rkv):
     assert lib.rkv_decode_mx4(None, C.byref(g), 72, 64, 8, 64, 2, C.byref(d), None) == -1 and "pages" in err()
     p = rkv.PrefillArgs()
     assert lib.rkv_prefill_mx4(None, C.byref(g), 72, 64, 8, 2, C.byref(p), None) == -1 and "pages" in err()
+
+
+def test_binding_refuses_other_memory(rkv):
+    """Rows over each other, and tensors of another device than the context's."""
+    import torch
+
+    class Cpu:
+        h, device = None, -1
+
+    class Gpu:
+        h, device = None, 0
+    f, pos = torch.ones(64), torch.zeros(3, dtype=torch.int32)
+    rope = rkv.rope_args(128, f, pos)
+    x = torch.zeros(3, 4, 128)
+    with pytest.raises(ValueError, match="follow each other"):
+        rkv.rope_rows(Cpu, rope, torch.zeros(1, 4, 128).expand(3, 4, 128), None, x, None, stream=0)
+    with pytest.raises(ValueError, match="rope"):
+        rkv.rope_rows(Gpu, rope, x, None, x, None, stream=0)
+    g = rkv.geometry(4, 128, 32, 3)
+    bt, pages = torch.zeros(1, 1, dtype=torch.int32), torch.zeros(64, dtype=torch.uint8)
+    over = torch.zeros(516).as_strided((3, 4, 128), (2, 128, 1))
+    with pytest.raises(ValueError, match="follow each other"):
+        rkv.append_rope(Cpu, g, rkv.CACHE_MX4, pages, bt, pos, pos, x, over, stream=0)
+    with pytest.raises(ValueError, match="device 0"):
+        rkv.read_rows(Gpu, g, rkv.CACHE_MX4, pages, bt, pos, pos, None, None, stream=0)
+    with pytest.raises(ValueError, match="device 0"):
+        rkv.append_rope(Gpu, g, rkv.CACHE_MX4, pages, bt, pos, pos, x, x, stream=0)
+    # what fits reaches the library, which refuses the missing context
+    buf = torch.zeros(4096, dtype=torch.uint8)
+    pages = buf[-buf.data_ptr() % 16:]
+    for call in (lambda: rkv.rope_rows(Cpu, rope, x, None, x, None, stream=0),
+                 lambda: rkv.append_rope(Cpu, g, rkv.CACHE_MX4, pages, bt, pos, pos, x, x, rope, stream=0),
+                 lambda: rkv.read_rows(Cpu, g, rkv.CACHE_MX4, pages, bt, pos, pos, x, None, stream=0)):
+        with pytest.raises(rkv.RkvError, match="ctx is NULL"):
+            call()

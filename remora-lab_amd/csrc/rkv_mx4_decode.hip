@@ -34,8 +34,8 @@
 // sequence of 262,145 tokens 35 us, 16 of 4k..16k 26, one of 300 8: locating
 // the partition, its page ids and its first tile come one after the other, and
 // a second launch joins partials (4.5 us).  32 x 32k tokens of 32 rows 131 us
-// (memory alone 83): 2 waves a SIMD issue 290 vector and 96 matrix instructions
-// a tile.  Not faster: two tiles in flight, a third wave a SIMD, 8 waves a
+// (memory alone 83): 2 waves a SIMD issue 380 vector and 96 matrix instructions
+// a tile, counted.  Not faster: two tiles in flight, a third wave a SIMD, 8 waves a
 // workgroup.
 #include <algorithm>
 

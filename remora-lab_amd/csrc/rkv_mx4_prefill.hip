@@ -18,9 +18,9 @@
 //     buffers, one barrier a tile.
 // Bound by issue: besides a 16-cycle matrix instruction a SIMD issues about two
 // others, from either of its two waves, and each further one costs 4.6 cycles.
-// A wave's tile takes 96 matrix instructions for f32 rows (64 for bf16) and 180
-// others at head_dim 256; widening V in every wave took 303 (804 us for the
-// first case below).  The queries' first half stays in registers and the second
+// A wave's tile takes 96 matrix instructions for f32 rows (64 for bf16) and 237
+// others at head_dim 256, counted; widening V in every wave took 357 (804 us
+// for the first case below).  The queries' first half stays in registers and the second
 // in LDS: both in LDS leave no room for two workgroups a CU, both in registers
 // spill.
 // Measured (2 kv heads of 256, 8 query heads each): eight chunks of 512 rows

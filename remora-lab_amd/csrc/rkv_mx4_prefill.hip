@@ -102,7 +102,7 @@ struct Mx4Block : Mx4Rows<D, 2, kTwo> {
         const uint32_t n0 = mx4_nans(s0), n1 = mx4_nans(s1);
         s0 &= ~((n0 >> 7) * 0xffu);
         s1 &= ~((n1 >> 7) * 0xffu);
-        auto bits = [](uint32_t n) { return n >> 7 & 1u | n >> 14 & 2u | n >> 21 & 4u | n >> 28 & 8u; };
+        auto bits = [](uint32_t n) { return (n >> 7 & 1u) | (n >> 14 & 2u) | (n >> 21 & 4u) | (n >> 28 & 8u); };
         if (li == 0)
           nan[(4 * buf + lg) * NB + b] = (uint8_t)(bits(n0) | bits(n1) << 4);
       }

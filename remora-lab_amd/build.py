@@ -24,8 +24,7 @@ SOURCES = ["rkv_append.hip", "rkv_decode.hip", "rkv_decode_rows32.hip", "rkv_mx4
 # two-wave 32-row variant (rkv_decode_rows32.hip) is bounded to 256 registers
 # per wave by its launch bounds and allocates no AGPRs either way.
 # rkv_mx4_decode.hip: without it the 17..32-row variant at head_dim 256 spills.
-EXTRA = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for f in ("rkv_decode.hip", "rkv_mx4_decode.hip",
-                                                            "rkv_mx4_prefill.hip")}
+EXTRA = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for f in ("rkv_decode.hip", "rkv_mx4_decode.hip")}
 
 # -packed-fp32-ops off: no v_pk_*_f32 are generated (unreliable on this pool).
 # f32 division and sqrt stay correctly rounded and f32 denormals are kept, so

@@ -193,6 +193,8 @@ struct Mx4Block : Mx4Rows<D, 2, kTwo> {
 };
 #endif  // __HIP_DEVICE_COMPILE__
 
+// Three waves a SIMD at head_dim 128, for 20 bytes of scratch a lane (eight
+// chunks of 1344 rows of 24 heads after 3000 tokens 648 us, with two 796).
 template <int D, bool kTwo>
 __global__ __launch_bounds__(64 * kMx4PrefillWaves, D == 128 ? 3 : 2) void mx4_prefill_kernel(PrefillLaunch pf) {
 #if defined(__HIP_DEVICE_COMPILE__)

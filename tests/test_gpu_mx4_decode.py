@@ -249,3 +249,33 @@ def test_captured_and_replayed(rkv, ctx):
         torch.cuda.synchronize()
         assert torch.equal(out, eager)
         assert torch.equal(run(rkv, ctx, c, q, 1 / 16), eager)
+
+
+def test_two_calls_at_once(rkv, ctx):
+    """Two streams, a workspace each, on the same pages and context: both give
+    the results of a call alone."""
+    import torch
+    c = Cache(rkv, 2, 256, 64, [3000, 40, 900, 2111], seed=41)
+    calls = []
+    for i in range(2):
+        q, _ = query((4, 1, 16, 256), 50 + i, True)
+        out = torch.empty(4, 1, 16, 256, device="cuda")
+        ids = torch.arange(4, dtype=torch.int32, device="cuda")
+        need = rkv.decode_mx4_workspace_bytes(c.g, rkv.decode_args(q, out, ids, 0.06, 3000))
+        assert need > 0
+        ws = torch.full((need,), 255, dtype=torch.uint8, device="cuda")
+        calls.append((rkv.decode_args(q, out, ids, 0.06, 3000, workspace=ws), q, out, ids, ws))
+    alone = []
+    for a, _, out, *_ in calls:
+        rkv.decode_mx4(ctx, c.g, c.pages, c.bt_d, c.lens_d, a)
+        ctx.sync()
+        alone.append(out.clone())
+        out.zero_()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    for _ in range(20):
+        for s, (a, *_) in zip(streams, calls):
+            rkv.decode_mx4(ctx, c.g, c.pages, c.bt_d, c.lens_d, a, stream=s)
+    torch.cuda.synchronize()
+    for want, (_, _, out, *_) in zip(alone, calls):
+        assert (out == want).all()

@@ -374,7 +374,9 @@ rkv_status rkv_decode_mx4(rkv_ctx *ctx, const rkv_kv_geometry *g, const void *pa
 size_t rkv_decode_mx4_workspace_bytes(const rkv_kv_geometry *g, const rkv_decode_args *args);
 
 /* rkv_prefill_q8 over 4-bit pages, with a bf16 query (q_dtype RKV_F32 is
- * RKV_ERR_UNSUPPORTED): the same arguments, split and faults.  f32 rows carry
+ * RKV_ERR_UNSUPPORTED): the same arguments and faults, and with segment_tokens
+ * 0 a split planned for this kernel (rkv_prefill_mx4_workspace_bytes says what
+ * it needs; a smaller workspace gets a coarser split or none).  f32 rows carry
  * their softmax weights in 22 bits, bf16 rows in 11.  NaN blocks as in
  * rkv_decode_mx4. */
 rkv_status rkv_prefill_mx4(rkv_ctx *ctx, const rkv_kv_geometry *g, const void *pages,
